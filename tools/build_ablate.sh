@@ -6,7 +6,7 @@ cd "$(dirname "$0")/.."
 mkdir -p ablate_build
 objs=$(ls diffusion-model_amd/csrc/build/*.o | grep -v conv3x3_halo)
 for m in "$@"; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics \
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops \
      -DDDPM_HALO_ABLATE=$m -x hip -c diffusion-model_amd/csrc/conv3x3_halo.hip -o ablate_build/halo_$m.o &
 done
 wait

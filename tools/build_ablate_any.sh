@@ -7,7 +7,7 @@ src=$1; macro=$2; shift 2
 mkdir -p ablate_build
 objs=$(ls diffusion-model_amd/csrc/build/*.o | grep -v "/$src\.")
 for m in "$@"; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics \
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops \
      -D$macro=$m -x hip -c diffusion-model_amd/csrc/$src.hip -o ablate_build/${src}_$m.o &
 done
 wait

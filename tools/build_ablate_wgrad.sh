@@ -6,7 +6,7 @@ cd "$(dirname "$0")/.."
 mkdir -p ablate_build
 objs=$(ls diffusion-model_amd/csrc/build/*.o | grep -v conv_wgrad)
 for m in "$@"; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics \
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops \
      -DDDPM_WG_ABLATE=$m -x hip -c diffusion-model_amd/csrc/conv_wgrad.hip -o ablate_build/wg_$m.o &
 done
 wait

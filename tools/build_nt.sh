@@ -9,7 +9,7 @@ mkdir -p ablate_build
 pat=$(echo $files | sed 's/ /\\|/g')
 objs=$(ls diffusion-model_amd/csrc/build/*.o | grep -v "/\($pat\)\.o")
 for f in $files; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics \
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -fno-gpu-rdc -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops \
      -DDDPM_STORE_AUX=$aux -x hip -c diffusion-model_amd/csrc/$f.hip -o ablate_build/${f}_nt.o &
 done
 wait

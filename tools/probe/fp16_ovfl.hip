@@ -1,7 +1,7 @@
 // Probe: MODE.FP16_OVFL (bit 23 of the MODE hardware register). With the bit set, a float -> fp16 conversion that
 // overflows gives +-65504 instead of infinity (true infinities and NaNs pass through). Prints the conversions of a few
 // values with the bit clear and set.
-// Build: hipcc --offload-arch=gfx950 -O3 -o fp16_ovfl fp16_ovfl.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o fp16_ovfl fp16_ovfl.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

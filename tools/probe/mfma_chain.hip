@@ -1,6 +1,6 @@
 // Probe: rate of v_mfma_f32_32x32x16_bf16 when consecutive instructions accumulate into the SAME registers
 // (a dependent chain) against 2 and 4 accumulators taken in turn, at one and two waves per SIMD.
-// Build: hipcc --offload-arch=gfx950 -O3 -o mfma_chain mfma_chain.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_chain mfma_chain.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

@@ -1,7 +1,7 @@
 // Probe: sustained rate of v_mfma_f32_32x32x16_bf16 when the operands change from one instruction to
 // the next (8 operand register sets of pseudo-random data) against constant operands: the chip's clock
 // under dense matrix work depends on how much the multiplier inputs toggle.
-// Build: hipcc --offload-arch=gfx950 -O3 -o mfma_power mfma_power.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_power mfma_power.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

@@ -1,6 +1,6 @@
 // Probe: do VALU instructions issue while the matrix pipe executes v_mfma_f32_32x32x16_bf16?
 // Each wave runs ITER rounds of 4 independent MFMAs interleaved with K independent v_fma_f32.
-// Build: hipcc --offload-arch=gfx950 -O3 -o mfma_valu_overlap mfma_valu_overlap.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_valu_overlap mfma_valu_overlap.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
