@@ -490,7 +490,7 @@ class Job:
                 par = (f"dp{world}: {backend} all-reduce of {args.bucket_mb} MiB gradient buckets launched from inside the backward"
                        if args.allreduce == "bucketed" else f"dp{world}: {backend} all-reduce of the flattened gradients after the backward")
             cfg.update(optimizer=("torch.optim.Adam(lr=2e-4)" if args.optimizer == "torch" else
-                                  "Adam(lr=2e-4), torch.optim.Adam's update as one HIP launch per 64 tensors"),
+                                  "Adam(lr=2e-4), torch.optim.Adam's update as one HIP launch per 88 tensors"),
                        batchnorm=bn, parallelism=par, last_loss=round(self.state["loss"], 5))
         # memory-side bytes per launch of the dominant kernel: not measurable live (hardware counters need their own
         # rocprofv3 --pmc passes), so taken from the newest committed summary of tools/pmc_traffic.sh for this workload

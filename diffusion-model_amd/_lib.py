@@ -91,6 +91,9 @@ _SIGNATURES = {
     "ddpm_inception_split_scores": [P, I64, I32, I32, P, P],
     "ddpm_mean_cov": [P, I64, I32, P, P, P, P],
     "ddpm_adam_step": [I32, P, P, P, P, P, F64, F64, F64, F64, F64, I64, P],
+    "ddpm_adam_step_clipped": [I32, P, P, P, P, P, F64, F64, F64, F64, F64, I64, P, P],
+    "ddpm_grad_norm": [I32, P, P, P, I32, F32, P, P, P],
+    "ddpm_clip_grads": [I32, P, P, P, P, P],
     "ddpm_conv3x3_fwd_stats": [C.POINTER(ConvDesc), P, P, P, C.POINTER(Epilogue), P, P, C.POINTER(C.c_int), P],
     "ddpm_bn_partials": [P, I32, I64, I32, P, C.POINTER(C.c_int), P],
     "ddpm_bn_stats_from_partials": [P, I32, I64, I32, F32, F32, P, P, P, P, P],
@@ -124,6 +127,8 @@ def lib():
         handle.ddpm_packed_weight_floats.argtypes = [I32, I32, I32]
         handle.ddpm_mean_cov_workspace_doubles.restype = C.c_int64
         handle.ddpm_mean_cov_workspace_doubles.argtypes = [I32]
+        handle.ddpm_grad_norm_workspace_doubles.restype = C.c_int64
+        handle.ddpm_grad_norm_workspace_doubles.argtypes = [I32]
         for name, sig in _SIGNATURES.items():
             fn = getattr(handle, name)          # AttributeError if the header and library disagree
             fn.argtypes = sig
@@ -133,7 +138,8 @@ def lib():
 
 
 def exported_symbols():
-    return ["ddpm_last_error", "ddpm_reduce_workspace_doubles", "ddpm_packed_weight_floats", "ddpm_mean_cov_workspace_doubles"] + list(_SIGNATURES)
+    return ["ddpm_last_error", "ddpm_reduce_workspace_doubles", "ddpm_packed_weight_floats", "ddpm_mean_cov_workspace_doubles",
+            "ddpm_grad_norm_workspace_doubles"] + list(_SIGNATURES)
 
 
 def packed_floats(taps, rows, cin):

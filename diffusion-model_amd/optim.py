@@ -1,19 +1,159 @@
 """`Adam`: torch.optim.Adam's update (the optimizer of the reference's training loops,
-first-iteration/main.py:51,82-84; third-iteration/main.py:61) as one HIP launch per 64 tensors.
+first-iteration/main.py:51,82-84; third-iteration/main.py:61) as one HIP launch per 88 tensors, and the global gradient
+norm with clipping by it: `clip_grad_norm_` / `grad_norm` in front of any optimizer, or `Adam(..., max_grad_norm=...)` /
+`adam_step_(..., max_norm=...)`, which scale the gradients as the update reads them instead of writing them first.
 
 Same constructor arguments, same per-parameter state (`step`, `exp_avg`, `exp_avg_sq`) and the same
 `state_dict()` layout as torch.optim.Adam, so optimizer checkpoints move both ways.  Parameters must be
 contiguous fp32 tensors on the GPU; there is no CPU fallback.
 """
 import ctypes as C
+import math
+from array import array
+from itertools import chain
+from operator import attrgetter
 
 import torch
 
-from ._lib import call
+from ._lib import call, lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # DDPM_F32, DDPM_BF16, DDPM_F16
+_NORMS = {2.0: 0, math.inf: 1}                                        # DDPM_NORM_2, DDPM_NORM_MAX
+_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_dtype, _device = attrgetter("dtype"), attrgetter("device")
+
+
+def _array(code, values):
+    """(address, owner) of a C array of `values`."""
+    a = array(code, values)
+    return C.c_void_p(a.buffer_info()[0]), a
+
+
+def _stream(device):
+    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _one_gpu(what, tensors):
+    devices = set(map(_device, tensors))
+    if len(devices) != 1 or next(iter(devices)).type != "cuda":
+        raise RuntimeError(f"{what} (HIP): all tensors must be on one GPU, got {sorted(map(str, devices))}")
+    return next(iter(devices))
+
+
+class _Norm:
+    """The gradients of one call as the C arrays of the norm and clipping entry points, and the norm itself:
+    `state` holds [norm, factor] on the device."""
+
+    def __init__(self, what, grads, max_norm, norm_type):
+        if norm_type not in _NORMS:
+            raise NotImplementedError(f"{what} (HIP): norm_type must be 2 or inf, got {norm_type}")
+        if not max_norm >= 0.0:
+            raise ValueError(f"Invalid max_norm: {max_norm}")
+        self.device = _one_gpu(what, grads)
+        if not all(map(_contiguous, grads)):
+            raise RuntimeError(f"{what} (HIP): gradients must be contiguous")
+        types = list(map(_TYPES.get, map(_dtype, grads)))
+        if None in types:
+            raise RuntimeError(f"{what} (HIP): gradients must be float32, bfloat16 or float16, got {sorted(map(str, set(map(_dtype, grads))))}")
+        self.n = len(grads)
+        numel = list(map(_numel, grads))
+        pointers = list(map(_ptr, grads))
+        if len(set(pointers)) < self.n and len({p for p, k in zip(pointers, numel) if k}) < sum(map(bool, numel)):
+            raise ValueError(f"{what} (HIP): the same gradient is given twice")
+        (self.pointers, a), (self.numel, b), (self.types, c) = _array("Q", pointers), _array("q", numel), _array("i", types)
+        self._owners = (a, b, c)
+        with torch.cuda.device(self.device):
+            workspace = torch.empty(lib().ddpm_grad_norm_workspace_doubles(self.n), dtype=torch.float64, device=self.device)
+            self.state = torch.empty(2, dtype=torch.float32, device=self.device)
+            call("ddpm_grad_norm", self.n, self.pointers, self.numel, self.types, _NORMS[norm_type], float(max_norm),
+                 C.c_void_p(workspace.data_ptr()), C.c_void_p(self.state.data_ptr()), _stream(self.device))
+
+    def factor(self):
+        return C.c_void_p(self.state.data_ptr() + 4)
+
+
+def _gradients(what, parameters):
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if any(g.is_sparse for g in grads):
+        raise RuntimeError(f"{what} does not support sparse gradients")
+    return grads
+
+
+@torch.no_grad()
+def grad_norm(parameters, norm_type=2.0):
+    """Norm of all gradients of `parameters` together (a 0-dim fp32 tensor on their GPU): the 2-norm, summed in float64
+    in a fixed order, or with norm_type=inf the largest magnitude. The gradients stay as they are."""
+    grads = [g if g.is_contiguous() else g.contiguous() for g in _gradients("grad_norm", parameters)]
+    return _Norm("grad_norm", grads, math.inf, float(norm_type)).state[0] if grads else torch.tensor(0.0)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ over fp32, bf16 and fp16 gradients on one GPU: scales all of them in place by
+    min(1, max_norm / (norm + 1e-6)) and returns the norm before (0-dim fp32, on the device; nothing waits for it unless
+    error_if_nonfinite is set). A norm that is not a number makes every gradient NaN, as there."""
+    grads = _gradients("clip_grad_norm_", parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    norm = _Norm("clip_grad_norm_", dense, max_norm, float(norm_type))
+    if error_if_nonfinite and not math.isfinite(norm.state[0].item()):
+        raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
+    with torch.cuda.device(norm.device):
+        call("ddpm_clip_grads", norm.n, norm.pointers, norm.numel, norm.types, norm.factor(), _stream(norm.device))
+        for g, d in zip(grads, dense):
+            if g is not d:
+                g.copy_(d)
+    torch.autograd.graph.increment_version(grads)
+    return norm.state[0]
+
+
+def _update(lists, step, lr, beta1, beta2, eps, weight_decay, factor):
+    """Launches the update of checked lists (parameters, gradients, exp_avg, exp_avg_sq) on the current GPU and stream."""
+    arrays = [_array("Q", map(_ptr, x)) for x in lists]
+    numel = _array("q", map(_numel, lists[0]))
+    args = (len(lists[0]), *(a[0] for a in arrays), numel[0], float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), step)
+    if factor is None:
+        call("ddpm_adam_step", *args, _stream(lists[0][0].device))
+    else:
+        call("ddpm_adam_step_clipped", *args, factor, _stream(lists[0][0].device))
+    # the kernel wrote the tensors behind autograd's back: record the in-place change, as any in-place
+    # torch op would (saved-tensor checks and caches keyed on the version counter rely on it)
+    torch.autograd.graph.increment_version(list(chain(lists[0], lists[2], lists[3])))
+
+
+@torch.no_grad()
+def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, max_norm=None):
+    """One Adam update of lists of contiguous fp32 tensors on one GPU, in place; `step` counts from 1, this update
+    included. With max_norm the gradients count as if clip_grad_norm_(max_norm) had scaled them first; they themselves stay
+    as they are, and their norm is returned (0-dim fp32 on the device; None without max_norm)."""
+    params, grads, exp_avgs, exp_avg_sqs = lists = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs)]
+    if len(set(map(len, lists))) != 1:
+        raise ValueError(f"adam_step_: lists of different lengths {[len(x) for x in lists]}")
+    if step < 1:
+        raise ValueError(f"Invalid step: {step}")
+    if not params:
+        return None
+    every = list(chain(*lists))
+    device = _one_gpu("adam_step_", every)
+    if set(map(_dtype, every)) != {torch.float32} or not all(map(_contiguous, every)):
+        raise RuntimeError("adam_step_ (HIP): all tensors must be contiguous fp32")
+    if any(len(set(x)) != 1 for x in zip(*(map(_numel, x) for x in lists))):
+        raise RuntimeError("adam_step_ (HIP): gradients and moments must match their parameters in size")
+    written = [t.data_ptr() for t in chain(params, exp_avgs, exp_avg_sqs) if t.numel()]
+    if len(set(written)) < len(written):
+        raise ValueError("adam_step_ (HIP): the same tensor is given twice")
+    norm = _Norm("adam_step_", grads, max_norm, 2.0) if max_norm is not None else None
+    with torch.cuda.device(device):
+        _update(lists, int(step), lr, *betas, eps, weight_decay, norm and norm.factor())
+    return norm and norm.state[0]
 
 
 class Adam(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, amsgrad=False, *, maximize=False):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, amsgrad=False, *, maximize=False,
+                 max_grad_norm=None):
         if not 0.0 <= lr:
             raise ValueError(f"Invalid learning rate: {lr}")
         if not 0.0 <= eps:
@@ -26,7 +166,12 @@ class Adam(torch.optim.Optimizer):
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
         if amsgrad or maximize:
             raise NotImplementedError("amsgrad / maximize are not part of the reference's optimizer and are not implemented")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False))
+        # of the optimizer, not of its groups: the norm is that of all gradients together, and a state_dict keeps torch's keys
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None        # norm of the gradients of the last step (0-dim, on the device) with max_grad_norm
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -34,6 +179,7 @@ class Adam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        work = []
         for group in self.param_groups:
             by_step = {}
             for p in group["params"]:
@@ -53,16 +199,16 @@ class Adam(torch.optim.Optimizer):
                     st["step"] = torch.tensor(0.0, dtype=torch.float32)
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                st["step"] += 1
-                by_step.setdefault(int(st["step"].item()), []).append((p, g, st["exp_avg"], st["exp_avg_sq"]))
-            for step, items in by_step.items():
-                n = len(items)
-                arrays = [(C.c_void_p * n)(*[t[k].data_ptr() for t in items]) for k in range(4)]
-                numel = (C.c_int64 * n)(*[t[0].numel() for t in items])
-                b1, b2 = group["betas"]
-                call("ddpm_adam_step", n, *arrays, numel, float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-                     float(group["weight_decay"]), step, C.c_void_p(torch.cuda.current_stream(items[0][0].device).cuda_stream))
-                # the kernel wrote the tensors behind autograd's back: record the in-place change, as any in-place
-                # torch op would (saved-tensor checks and caches keyed on the version counter rely on it)
-                torch.autograd.graph.increment_version([t[k] for t in items for k in (0, 2, 3)])
+                by_step.setdefault(int(st["step"].item()) + 1, []).append((p, g, st["exp_avg"], st["exp_avg_sq"]))
+            work += [(group, step, items) for step, items in by_step.items()]
+        norm = None
+        if self.max_grad_norm is not None and work:
+            norm = _Norm("Adam", [t[1] for _, _, items in work for t in items], self.max_grad_norm, 2.0)
+            self.grad_norm = norm.state[0]
+        for group, step, items in work:
+            with torch.cuda.device(items[0][0].device):
+                _update([list(x) for x in zip(*items)], step, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
+                        norm and norm.factor())
+            for p, *_ in items:
+                self.state[p]["step"] += 1
         return loss

@@ -35,6 +35,11 @@ extern "C" {
 #define DDPM_E_INVALID (-1)  /* bad argument / unsupported shape */
 #define DDPM_E_LAUNCH (-2)   /* HIP reported an error at launch   */
 
+/* Element types of the entry points that take more than fp32. */
+#define DDPM_F32 0
+#define DDPM_BF16 1
+#define DDPM_F16 2
+
 #define DDPM_ACT_NONE 0
 #define DDPM_ACT_RELU 1 /* first-iteration/unet.py:18,21 */
 #define DDPM_ACT_GELU 2 /* exact erf GELU, second-iteration/unet.py:19,26,35 */
@@ -170,6 +175,27 @@ int ddpm_range_flag_read(uint32_t* host_dst, int clear, void* stream);
 int ddpm_adam_step(int ntensors, float* const* params, const float* const* grads, float* const* exp_avg,
                    float* const* exp_avg_sq, const int64_t* numel, double lr, double beta1, double beta2,
                    double eps, double weight_decay, int64_t step, void* stream);
+
+/* Norm of a list of gradients taken together, and clipping by it: what a training loop puts between backward and
+ * optimizer step (loss.backward(); optimizer.step(), first-iteration/main.py:83-84; the reference does not clip). Host
+ * arrays of ntensors device pointers (aligned to their elements), element counts and DDPM_F32 / BF16 / F16 codes, consumed
+ * before the call returns; a gradient must not be listed twice.
+ *   ddpm_grad_norm: state[0] = norm (DDPM_NORM_2: square root of the float64 sum of squares; DDPM_NORM_MAX: largest
+ *     magnitude; NaN when a gradient is), state[1] = min(1, max_norm / (norm + 1e-6)), two device floats. The same
+ *     gradients give the same bits. workspace: ddpm_grad_norm_workspace_doubles(ntensors) doubles.
+ *   ddpm_clip_grads: every gradient times factor[0] (device), in place, rounded to its own type.
+ *   ddpm_adam_step_clipped: ddpm_adam_step with every gradient times factor[0] (device) as it is read; the gradients
+ *     themselves stay as they are. */
+#define DDPM_NORM_2 0
+#define DDPM_NORM_MAX 1
+int64_t ddpm_grad_norm_workspace_doubles(int ntensors);
+int ddpm_grad_norm(int ntensors, const void* const* grads, const int64_t* numel, const int32_t* types, int kind,
+                   float max_norm, double* workspace, float* state, void* stream);
+int ddpm_clip_grads(int ntensors, void* const* grads, const int64_t* numel, const int32_t* types, const float* factor,
+                    void* stream);
+int ddpm_adam_step_clipped(int ntensors, float* const* params, const float* const* grads, float* const* exp_avg,
+                           float* const* exp_avg_sq, const int64_t* numel, double lr, double beta1, double beta2,
+                           double eps, double weight_decay, int64_t step, const float* factor, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * Time / label embedding: sinusoidal embedding followed by the four time Linears (and, when
