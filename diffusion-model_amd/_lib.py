@@ -35,6 +35,12 @@ class EmbedArgs(C.Structure):
                 ("out", P * 4), ("emb_out", P)]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [("type", I32), ("batch", I32), ("tokens", I32), ("dim", I32), ("axes", I32), ("axis_dim", I32 * 4), ("interleaved", I32),
+                ("inverse", I32), ("position_type", I32), ("tensors", I32), ("heads", I32 * 2), ("base", F64), ("positions", P),
+                ("position_batch_stride", I64), ("x", P * 2), ("out", P * 2), ("x_stride", (I64 * 3) * 2), ("out_stride", (I64 * 3) * 2)]
+
+
 _SIGNATURES = {
     "ddpm_abi_version": [],
     "ddpm_schedule_betas": [I32, I32, F64, F64, P],
@@ -50,6 +56,7 @@ _SIGNATURES = {
     "ddpm_mse_fwd": [P, P, I64, P, P, P],
     "ddpm_mse_bwd": [P, P, P, I64, P, P],
     "ddpm_time_embed": [C.POINTER(EmbedArgs), P],
+    "ddpm_rotary": [C.POINTER(RotaryArgs), P],
     "ddpm_sinusoidal_embedding": [P, I32, I32, I32, P, P],
     "ddpm_conv3x3_fwd": [C.POINTER(ConvDesc), P, P, P, C.POINTER(Epilogue), P, P],
     "ddpm_conv1x1_fwd": [C.POINTER(ConvDesc), P, P, P, C.POINTER(Epilogue), P, P],

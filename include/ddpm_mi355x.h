@@ -39,6 +39,8 @@ extern "C" {
 #define DDPM_F32 0
 #define DDPM_BF16 1
 #define DDPM_F16 2
+#define DDPM_I32 3
+#define DDPM_I64 4
 
 #define DDPM_ACT_NONE 0
 #define DDPM_ACT_RELU 1 /* first-iteration/unet.py:18,21 */
@@ -230,6 +232,35 @@ int ddpm_time_embed(const ddpm_embed_args* a, void* stream);
 /* The sinusoidal embedding alone: out[b] = [sin(t_b*f_k) | cos(t_b*f_k)], f_k = exp(-k*ln(1e4)/(E/2-1)),
  * written as [batch][2*(E/2)]. Replaces SinusoidalTimeEmbedding.forward, first-iteration/embeddings.py:11-20. */
 int ddpm_sinusoidal_embedding(const void* t, int t_is_float, int batch, int emb_dim, float* out, void* stream);
+
+/* Rotary positions with several axes (time, height, width; one for a plain sequence): pair i of the axis_dim[a] channels
+ * of axis a is turned by positions[token][a] * base^(-2 i / axis_dim[a]); the axes own consecutive channels from 0 on, and
+ * channels behind the last axis pass unchanged. A pair is (i, axis_dim/2 + i) within its axis, or (2 i, 2 i + 1) with
+ * interleaved != 0. inverse != 0 turns back: the gradient of the forward call. Angles are formed and reduced in float64.
+ * One or two tensors (queries and keys of one sequence, own head counts) with the same positions; element (b, n, h, c) of
+ * tensor i lies at x[i] + b*x_stride[i][0] + n*x_stride[i][1] + h*x_stride[i][2] + c, so that a channel slice of a fused
+ * projection serves; out must not overlap x. positions: [batch or 1][tokens][axes], DDPM_I32, I64 or F32;
+ * position_batch_stride 0 shares them over the batch. Beside the reference's embedding of the timestep
+ * (first-iteration/embeddings.py:11-20), which has no counterpart for pixels. */
+#define DDPM_ROTARY_MAX_AXES 4
+#define DDPM_ROTARY_MAX_DIM 512
+typedef struct ddpm_rotary_args {
+    int32_t type;                    /* DDPM_F32, BF16, F16: of x and out */
+    int32_t batch, tokens, dim;      /* dim <= DDPM_ROTARY_MAX_DIM */
+    int32_t axes;                    /* 1 ... DDPM_ROTARY_MAX_AXES */
+    int32_t axis_dim[4];             /* even, >= 2, together <= dim */
+    int32_t interleaved, inverse;
+    int32_t position_type;           /* DDPM_I32, I64, F32 */
+    int32_t tensors;                 /* 1 or 2 */
+    int32_t heads[2];
+    double base;                     /* > 1 */
+    const void* positions;
+    int64_t position_batch_stride;   /* elements */
+    const void* x[2];
+    void* out[2];
+    int64_t x_stride[2][3], out_stride[2][3];   /* elements: batch, token, head */
+} ddpm_rotary_args;
+int ddpm_rotary(const ddpm_rotary_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * Convolutions as implicit GEMM on the matrix cores, LDS-staged tiles.

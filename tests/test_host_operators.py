@@ -65,3 +65,54 @@ def test_clipping_functions_refuse_before_the_gpu():
     with pytest.raises(ValueError, match="step"):
         optim.adam_step_(t, t, t, t, 0)
     assert optim.adam_step_([], [], [], [], 1, max_norm=1.0) is None
+
+
+def _rotary_args(at, **change):
+    a = _lib.RotaryArgs()
+    a.type, a.batch, a.tokens, a.dim, a.axes, a.tensors, a.base, a.position_type = 0, 1, 2, 16, 2, 2, 1e4, 3
+    a.axis_dim[:2] = (8, 8)
+    a.heads[:] = (1, 1)
+    a.positions = at
+    a.x[:], a.out[:] = (at, at + 16), (at + 32, at + 48)
+    for k, v in change.items():
+        if isinstance(v, tuple):
+            getattr(a, k)[v[0]] = v[1]
+        else:
+            setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change", [dict(type=3), dict(position_type=1), dict(batch=-1), dict(tokens=-1), dict(dim=0), dict(dim=514), dict(dim=8),
+                                    dict(axes=0), dict(axes=5), dict(axis_dim=(0, 7)), dict(axis_dim=(0, 0)), dict(axis_dim=(1, 10)),
+                                    dict(tensors=0), dict(tensors=3), dict(base=1.0), dict(base=math.inf), dict(base=math.nan), dict(positions=None),
+                                    dict(x=(1, None)), dict(out=(0, None)), dict(heads=(1, 0)), dict(heads=(0, 70000))])
+def test_rotary_refuses(change):
+    keep, base = _aligned()
+    assert _lib.lib().ddpm_rotary(C.byref(_rotary_args(base, **change)), None) == -1
+    assert _lib.lib().ddpm_last_error()
+
+
+def test_rotary_refuses_overlap_null_and_misaligned():
+    keep, base = _aligned()
+    L = _lib.lib()
+    assert L.ddpm_rotary(None, None) == -1
+    assert L.ddpm_rotary(C.byref(_rotary_args(base, out=(0, base))), None) == -1
+    assert L.ddpm_rotary(C.byref(_rotary_args(base, x=(0, base + 2))), None) == -1
+    assert L.ddpm_rotary(C.byref(_rotary_args(base, batch=0)), None) == 0          # nothing to do
+
+
+def test_rotary_function_refuses():
+    from diffusion_model_amd.embedding import grid_positions, rotary
+    q, k, pos = torch.zeros(2, 6, 4, 16), torch.zeros(2, 6, 2, 16), grid_positions(2, 3, device="cpu")
+    assert pos.tolist() == [[0, 0], [0, 1], [0, 2], [1, 0], [1, 1], [1, 2]]
+    for args, error in (((q[0], k, pos, (8, 8)), ValueError), ((q, k.double(), pos, (8, 8)), TypeError), ((q.double(), None, pos, (8, 8)), TypeError),
+                        ((q, k[:, :5], pos, (8, 8)), ValueError), ((q, k, pos, (8, 10)), ValueError), ((q, k, pos, (7, 8)), ValueError),
+                        ((q, k, pos, ()), ValueError), ((q, k, pos, (16,)), ValueError), ((q, k, pos[:5], (8, 8)), ValueError),
+                        ((q, k, pos.double(), (8, 8)), TypeError), ((q, k, pos.float().requires_grad_(True), (8, 8)), TypeError),
+                        ((q, k, pos, (8, 8)), RuntimeError), ((torch.zeros(1, 6, 1, 514), None, pos, (8, 8)), ValueError)):
+        with pytest.raises(error):
+            rotary(*args)
+    with pytest.raises(ValueError):
+        grid_positions()
+    with pytest.raises(ValueError):
+        grid_positions(3, 0, device="cpu")
