@@ -41,6 +41,15 @@ class RotaryArgs(C.Structure):
                 ("position_batch_stride", I64), ("x", P * 2), ("out", P * 2), ("x_stride", (I64 * 3) * 2), ("out_stride", (I64 * 3) * 2)]
 
 
+class SpanAttentionArgs(C.Structure):
+    _fields_ = [(n, I32) for n in ("type", "batch", "nq", "nk", "heads", "kv_heads", "dim", "causal")] + \
+               [("scale", F32), ("softcap", F32), ("slopes", P), ("spans", P), ("positions", P), ("span_batch_stride", I64),
+                ("position_batch_stride", I64), ("q", P), ("k", P), ("v", P), ("out", P), ("lse", P)] + \
+               [(n, I64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
+               [(n, P) for n in ("dout", "dq", "dk", "dv")] + \
+               [(n, I64 * 3) for n in ("dout_stride", "dq_stride", "dk_stride", "dv_stride")]
+
+
 _SIGNATURES = {
     "ddpm_abi_version": [],
     "ddpm_schedule_betas": [I32, I32, F64, F64, P],
@@ -94,6 +103,8 @@ _SIGNATURES = {
     "ddpm_attention_bwd": [P, P, I32, P, P, P, P, P, P, P, I32, I32, I32, I32, P],
     "ddpm_attention_fwd": [P, P, I32, P, P, I32, P, P, P, I32, I32, I32, I32, P],
     "ddpm_self_attention_infer": [P, I32, P, P, P, P, P, I32, P, I32, I32, I32, I32, P],
+    "ddpm_span_attention_fwd": [C.POINTER(SpanAttentionArgs), P, P],
+    "ddpm_span_attention_bwd": [C.POINTER(SpanAttentionArgs), P, P],
     "ddpm_softmax_rows": [P, I64, I32, P, P],
     "ddpm_inception_split_scores": [P, I64, I32, I32, P, P],
     "ddpm_mean_cov": [P, I64, I32, P, P, P, P],
@@ -136,6 +147,9 @@ def lib():
         handle.ddpm_mean_cov_workspace_doubles.argtypes = [I32]
         handle.ddpm_grad_norm_workspace_doubles.restype = C.c_int64
         handle.ddpm_grad_norm_workspace_doubles.argtypes = [I32]
+        for name in ("ddpm_span_attention_fwd_workspace", "ddpm_span_attention_bwd_workspace"):
+            getattr(handle, name).restype = C.c_int64
+            getattr(handle, name).argtypes = [C.POINTER(SpanAttentionArgs)]
         for name, sig in _SIGNATURES.items():
             fn = getattr(handle, name)          # AttributeError if the header and library disagree
             fn.argtypes = sig
@@ -146,7 +160,7 @@ def lib():
 
 def exported_symbols():
     return ["ddpm_last_error", "ddpm_reduce_workspace_doubles", "ddpm_packed_weight_floats", "ddpm_mean_cov_workspace_doubles",
-            "ddpm_grad_norm_workspace_doubles"] + list(_SIGNATURES)
+            "ddpm_grad_norm_workspace_doubles", "ddpm_span_attention_fwd_workspace", "ddpm_span_attention_bwd_workspace"] + list(_SIGNATURES)
 
 
 def packed_floats(taps, rows, cin):

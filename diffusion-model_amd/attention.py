@@ -1,0 +1,194 @@
+"""Span attention: several heads, keys and values shared by groups of query heads, scores capped by a tanh, a bias by
+distance, and masks in which every row sees one span of keys (documents packed into a sequence, prefixes, padded lengths,
+windows, causal order), with its gradient. It stands beside the UNet's own self-attention (second-iteration/unet.py:39-61: one
+head, every pixel sees every pixel) for networks over tokens of images, video and text."""
+import ctypes as C
+
+import torch
+
+from ._lib import SpanAttentionArgs, call, lib
+
+_TYPES = {torch.float32: (0, 4), torch.bfloat16: (1, 8), torch.float16: (2, 8)}      # DDPM_* code, elements of 16 bytes
+MAX_DIM = 128
+
+
+def key_spans(rows, keys=None, *, documents=None, prefix=None, lengths=None, window=None, causal=False, device=None):
+    """Spans [first, last) of keys that each of `rows` rows sees, int32 [batch or 1][rows][2], for span_attention. Row i stands at
+    position i + keys - rows; every condition given narrows what it sees:
+      documents  [batch][keys] or [keys], any integers: a document is a run of equal ones; rows see their own document
+      causal     no key behind the row's position
+      prefix     an int or [batch]: causal, but all see the first `prefix` keys (of their document)
+      lengths    [batch]: keys from lengths[b] on hold nothing, and rows that stand there see nothing
+      window     (left, right): keys at most that far before and behind the row's position"""
+    keys = rows if keys is None else keys
+    if rows < 0 or keys < 0:
+        raise ValueError(f"key_spans: {rows} rows, {keys} keys")
+    if device is None:
+        given = [t.device for t in (documents, prefix, lengths) if isinstance(t, torch.Tensor)]
+        device = given[0] if given else "cuda"
+    at = torch.arange(rows, device=device)[None] + (keys - rows)
+    first, last = torch.zeros_like(at), torch.full_like(at, keys)
+    if documents is not None:
+        d = documents.to(device)
+        d = d[None] if d.dim() == 1 else d
+        if d.dim() != 2 or d.shape[1] != keys:
+            raise ValueError(f"key_spans: documents are [batch][{keys}], got {tuple(documents.shape)}")
+        j = torch.arange(keys, device=device).expand_as(d)
+        new = torch.ones_like(d, dtype=torch.bool)
+        new[:, 1:] = d[:, 1:] != d[:, :-1]
+        begin = torch.where(new, j, 0).cummax(1).values if keys else j
+        stop = torch.where(new, j, keys).roll(-1, 1) if keys else j
+        if keys:
+            stop[:, -1] = keys
+            stop = stop.flip(1).cummin(1).values.flip(1)
+        own = at.clamp(0, max(keys - 1, 0)).expand(d.shape[0], rows)
+        inside = (at >= 0) & (at < keys)
+        first = begin.gather(1, own)
+        last = torch.where(inside, stop.gather(1, own), first)
+    if prefix is not None:
+        p = prefix.to(device).reshape(-1, 1) if isinstance(prefix, torch.Tensor) else torch.tensor([[prefix]], device=device)
+        last = torch.minimum(last, torch.maximum(at + 1, first + p))
+    if causal:
+        last = torch.minimum(last, at + 1)
+    if window is not None:
+        left, right = window
+        first = torch.maximum(first, at - left)
+        last = torch.minimum(last, at + right + 1)
+    if lengths is not None:
+        n = lengths.to(device).reshape(-1, 1)
+        last = torch.where(at < n, torch.minimum(last, n), 0)
+    first, last = torch.broadcast_tensors(first, torch.maximum(last, first))
+    return torch.stack([first, last], -1).to(torch.int32)
+
+
+def _fit(x, width):
+    """x, or a copy, with neighbouring channels on 16-byte boundaries."""
+    if x.stride(3) != 1 or x.data_ptr() % 16 or any(n > 1 and s % width for n, s in zip(x.shape[:3], x.stride())):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _put(a, name, x, stride):
+    setattr(a, name, x.data_ptr())
+    getattr(a, stride)[:] = [s if n > 1 else 0 for n, s in zip(x.shape[:3], x.stride())]
+
+
+def _arguments(q, k, v, out, lse, how):
+    scale, softcap, slopes, spans, positions, causal = how
+    a = SpanAttentionArgs()
+    a.type = _TYPES[q.dtype][0]
+    a.batch, a.nq, a.heads, a.dim = q.shape
+    a.nk, a.kv_heads = k.shape[1], k.shape[2]
+    a.causal, a.scale, a.softcap = causal, scale, softcap
+    if slopes is not None:
+        a.slopes = slopes.data_ptr()
+    if spans is not None:
+        a.spans, a.span_batch_stride = spans.data_ptr(), spans.stride(0) if spans.shape[0] > 1 else 0
+    if positions is not None:
+        a.positions, a.position_batch_stride = positions.data_ptr(), positions.stride(0) if positions.shape[0] > 1 else 0
+    _put(a, "q", q, "q_stride")
+    _put(a, "k", k, "k_stride")
+    _put(a, "v", v, "v_stride")
+    _put(a, "out", out, "out_stride")
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    return a
+
+
+def _run(entry, a, device):
+    size = getattr(lib(), entry + "_workspace")(C.byref(a))
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+    call(entry, C.byref(a), C.c_void_p(workspace.data_ptr() if size > 0 else None), C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+
+
+def _forward(q, k, v, how, with_lse):
+    width = _TYPES[q.dtype][1]
+    q, k, v = (_fit(x, width) for x in (q, k, v))
+    with torch.cuda.device(q.device):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if with_lse else None
+        _run("ddpm_span_attention_fwd", _arguments(q, k, v, out, lse, how), q.device)
+    return q, k, v, out, lse
+
+
+class _SpanAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, softcap, slopes, spans, positions, causal):
+        q, k, v, out, lse = _forward(q, k, v, (scale, softcap, slopes, spans, positions, causal), True)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, spans, positions)
+        ctx.how = scale, softcap, causal
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, out, lse, slopes, spans, positions = ctx.saved_tensors
+        scale, softcap, causal = ctx.how
+        dout = _fit(dout, _TYPES[q.dtype][1])
+        with torch.cuda.device(q.device):
+            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+            a = _arguments(q, k, v, out, lse, (scale, softcap, slopes, spans, positions, causal))
+            _put(a, "dout", dout, "dout_stride")
+            _put(a, "dq", dq, "dq_stride")
+            _put(a, "dk", dk, "dk_stride")
+            _put(a, "dv", dv, "dv_stride")
+            _run("ddpm_span_attention_bwd", a, q.device)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None, positions=None, causal=False, return_lse=False):
+    """softmax(w) v over the keys that each row sees, w = softcap tanh(scale q.k / softcap) - slope |position - j|.
+
+    q: [batch][rows][heads][dim]; k, v: [batch][keys][kv_heads][dim] with heads a multiple of kv_heads (query head h uses
+    key/value head h // (heads / kv_heads)); float32, bfloat16 or float16, dim at most 128, any strides (16-byte aligned
+    ones are used in place, others through a copy).
+      scale      of q.k; dim ** -0.5 when not given          softcap    0: no cap
+      slopes     float32 [heads], or None: no bias           causal     row i sees no key behind its position
+      spans      int32 [batch or 1][rows][2]: the keys [first, last) of each row (key_spans makes them), or None: all
+      positions  int32 [rows] or [batch or 1][rows]; row i stands at i + keys - rows when not given
+    A row that sees no key comes out as noughts. Single tokens against long keys (rows = 1, one span each) are split over
+    the GPU. Returns out [batch][rows][heads][dim], with return_lse also the log-sum-exp of w, float32
+    [batch][heads][rows] (-inf for a row that sees none), which has no gradient; q, k and v have one."""
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if x.dim() != 4:
+            raise ValueError(f"span_attention: {name} is [batch][tokens][heads][dim], got {tuple(x.shape)}")
+        if x.dtype not in _TYPES or x.dtype != q.dtype:
+            raise TypeError(f"span_attention: q, k and v are of one type, float32, bfloat16 or float16, got {q.dtype} and {x.dtype}")
+    batch, rows, heads, dim = q.shape
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim or k.shape[2] < 1 or heads < 1 or heads % k.shape[2]:
+        raise ValueError(f"span_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if not 1 <= dim <= MAX_DIM:
+        raise ValueError(f"span_attention: at most {MAX_DIM} channels a head, got {dim}")
+    if not 0.0 <= softcap < 1e30:
+        raise ValueError(f"span_attention: softcap must not be negative, got {softcap}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < 1e30:
+        raise ValueError(f"span_attention: scale must be finite, got {scale}")
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,):
+            raise ValueError(f"span_attention: slopes are float32 [{heads}], got {slopes.dtype} {tuple(slopes.shape)}")
+        if slopes.requires_grad:
+            raise NotImplementedError("span_attention: slopes have no gradient")
+        slopes = slopes.contiguous()
+    if spans is not None:
+        if spans.dtype != torch.int32 or tuple(spans.shape) not in ((batch, rows, 2), (1, rows, 2)):
+            raise ValueError(f"span_attention: spans are int32 [{batch} or 1][{rows}][2], got {spans.dtype} {tuple(spans.shape)}")
+        spans = spans.contiguous()
+    if positions is not None:
+        positions = positions[None] if positions.dim() == 1 else positions
+        if positions.dtype != torch.int32 or tuple(positions.shape) not in ((batch, rows), (1, rows)):
+            raise ValueError(f"span_attention: positions are int32 [{batch} or 1][{rows}], got {positions.dtype} {tuple(positions.shape)}")
+        positions = positions.contiguous()
+    if not all(x.is_cuda and x.device == q.device for x in (q, k, v, slopes, spans, positions) if x is not None):
+        raise RuntimeError("span_attention runs on the MI355X only: all tensors must be on one GPU")
+    spare = -dim % _TYPES[q.dtype][1]
+    if spare:                                                   # noughts fill the last 16 bytes of a head
+        q, k, v = (torch.nn.functional.pad(x, (0, spare)) for x in (q, k, v))
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v)):
+        out, lse = _SpanAttention.apply(q, k, v, scale, float(softcap), slopes, spans, positions, bool(causal))
+    else:
+        *_, out, lse = _forward(q, k, v, (scale, float(softcap), slopes, spans, positions, bool(causal)), return_lse)
+    if spare:
+        out = out[..., :dim].contiguous()
+    return (out, lse) if return_lse else out

@@ -1,0 +1,282 @@
+// Parts shared by the forward and backward kernels of span attention: how rows of a tensor meet the matrix instructions,
+// how tiles reach LDS, what a row sees, and how a score comes from a product.
+//
+// Everything is built from two products of a 32-row tile in LDS:
+//   dot:    X[row][col] = sum over channels of tile[row] and the lane's own row (held in registers),
+//   spread: Y[channel][col] += sum over tile rows of tile[row][channel] * weight[row][col],
+// with one column per lane (col = lane % 32). In the layout of the 32x32 results a lane holds 16 rows of its column,
+// register r of lane half h being row 8 (r / 4) + 4 h + r % 4, so the weights made from a dot's result are already where spread
+// wants its second operand: the sum over rows may run in any order, and the first operand is read from LDS in the order the
+// registers have. No score ever moves between lanes; a column's maximum and sum need one exchange between the lane halves.
+//   forward:  scores = dot(K, q), out += spread(V, p)                    columns are queries
+//   dq:       scores = dot(K, q), dp = dot(V, dout), dq += spread(K, ds)  columns are queries
+//   dk, dv:   scores = dot(Q, k), dp = dot(dOut, v), dv += spread(dOut, p), dk += spread(Q, ds)   columns are keys
+#pragma once
+#include "common.h"
+
+namespace span {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;            // 4 waves
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// running maximum before the first key: finite, so that its difference from -infinity (a masked score) is one
+constexpr float kNoMax = -1e30f;
+
+struct Strides {
+    int64_t batch, row, head;
+};
+
+struct Dev {
+    int nq, nk, heads, group, dim;       // group: query heads per key/value head
+    int causal;
+    float scale, softcap;
+    const float* slopes;
+    const int32_t* spans;
+    const int32_t* positions;
+    int64_t span_batch, position_batch;
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    Strides sq, sk, sv, so;
+    const void* dout;
+    void *dq, *dk, *dv;
+    Strides sdo, sdq, sdk, sdv;
+};
+
+// ---- what a row sees -----------------------------------------------------------------------------------------------
+struct Row {
+    int lo, hi, pos;                     // keys [lo, hi); lo = INT_MAX, hi = 0: none
+};
+
+__device__ __forceinline__ Row row_of(const Dev& a, int b, int i) {
+    Row r;
+    r.pos = a.positions ? a.positions[b * a.position_batch + i] : i + a.nk - a.nq;
+    r.lo = 0;
+    r.hi = a.nk;
+    if (a.spans) {
+        const int32_t* s = a.spans + b * a.span_batch + 2 * static_cast<int64_t>(i);
+        r.lo = max(s[0], 0);
+        r.hi = min(s[1], a.nk);
+    }
+    if (a.causal && r.pos < r.hi) r.hi = r.pos + 1;
+    if (r.hi <= r.lo) {
+        r.lo = INT32_MAX;
+        r.hi = 0;
+    }
+    return r;
+}
+
+__device__ __forceinline__ Row no_row() { return {INT32_MAX, 0, 0}; }
+
+// smallest lo and largest hi of the wave
+__device__ __forceinline__ void join_rows(int& lo, int& hi) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        lo = min(lo, __shfl_xor(lo, d));
+        hi = max(hi, __shfl_xor(hi, d));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+}
+
+// the other lane half's value of this column
+__device__ __forceinline__ float other_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---- matrix products of a type ---------------------------------------------------------------------------------------
+template <typename T>
+struct Ops {                             // bf16, fp16
+    typedef T Frag __attribute__((ext_vector_type(8)));
+    static constexpr int W = 8;          // elements of 16 bytes
+    static constexpr int kStep = 16;     // channels of one step of dot
+    static constexpr int kTile = 64;     // rows staged at a time
+    // Weights are scaled by 2^kShift before they are rounded to T: fp16 has no more than 2^-24 at its small end, and a row of
+    // thousands of keys has many weights below its normal numbers; bf16 has fp32's range.
+    static constexpr int kShift = __is_same(T, _Float16) ? 14 : 0;
+    struct Weights {
+        Frag f[2];
+    };
+
+    static __device__ __forceinline__ f32x16 mfma(Frag a, Frag b, f32x16 c) {
+        if constexpr (__is_same(T, _Float16))
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Weights pack(const f32x16& p) {
+        Weights w;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w.f[r >> 3][r & 7] = static_cast<T>(p[r]);
+        return w;
+    }
+    // acc[db] += over 32 tile rows; `tile` points at the first of them
+    template <int DP, int PITCH>
+    static __device__ __forceinline__ void spread(f32x16* acc, const T* tile, const Weights& w) {
+        // The transposing read gives lane l of 16 the column l of a 4 x 16 block whose rows four lanes each point at: rows
+        // 4 h ... 4 h + 3 (and 8 further) are the ones whose weights this lane half holds.
+        const int lane = threadIdx.x & 63, l16 = lane & 15;
+        const T* at = tile + (4 * (lane >> 5) + (l16 >> 2)) * PITCH + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) {
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4*)(at + 16 * t * PITCH + 32 * db));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4*)(at + (16 * t + 8) * PITCH + 32 * db));
+                const auto xy = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[db] = mfma(__builtin_bit_cast(Frag, xy), w.f[t], acc[db]);
+            }
+    }
+    static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) { return mfma(a, b, c); }
+};
+
+template <>
+struct Ops<float> {
+    typedef f32x4 Frag;
+    static constexpr int W = 4;
+    static constexpr int kStep = 8;
+    static constexpr int kTile = 32;
+    static constexpr int kShift = 0;
+    typedef f32x16 Weights;
+
+    static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ Weights pack(const f32x16& p) { return p; }
+    template <int DP, int PITCH>
+    static __device__ __forceinline__ void spread(f32x16* acc, const float* tile, const Weights& w) {
+        const int lane = threadIdx.x & 63;
+        const float* at = tile + 4 * (lane >> 5) * PITCH + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * PITCH + 32 * db], w[r], acc[db], 0, 0, 0);
+    }
+};
+
+// row pitch of a tile in LDS: 16 bytes beyond the row, so that the 32 rows a dot reads at once start in different banks
+template <typename T, int DP>
+constexpr int pitch() {
+    return DP + Ops<T>::W;
+}
+
+// the lane's own row: channels kStep s + W h ... of step s, nought behind dim
+template <typename T, int DP>
+struct OwnRow {
+    static constexpr int kSteps = DP / Ops<T>::kStep;
+    typename Ops<T>::Frag f[kSteps];
+
+    __device__ __forceinline__ void load(const T* row, int dim) {       // row == nullptr: noughts
+        const int c0 = Ops<T>::W * ((threadIdx.x >> 5) & 1);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = c0 + Ops<T>::kStep * s;
+            f[s] = typename Ops<T>::Frag{};
+            if (row && c < dim) f[s] = *reinterpret_cast<const typename Ops<T>::Frag*>(row + c);
+        }
+    }
+    // product with 32 tile rows
+    template <int PITCH>
+    __device__ __forceinline__ f32x16 dot(const T* tile) const {
+        const int lane = threadIdx.x & 63;
+        const T* at = tile + (lane & 31) * PITCH + Ops<T>::W * (lane >> 5);
+        f32x16 acc = {};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) acc = Ops<T>::mul(*reinterpret_cast<const typename Ops<T>::Frag*>(at + Ops<T>::kStep * s), f[s], acc);
+        return acc;
+    }
+};
+
+// kTile rows on their way from memory to LDS. Rows outside [lo, hi) read the nearest row inside: they are masked, and what
+// memory holds behind a sequence is not looked at. Channels behind dim become noughts.
+template <typename T, int DP>
+struct Staged {
+    static constexpr int kChunks = DP / Ops<T>::W, kLoads = Ops<T>::kTile * kChunks / kThreads;
+    typename Ops<T>::Frag r[kLoads];
+
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int lo, int hi, int dim) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, c = (idx - row * kChunks) * Ops<T>::W;
+            const int at = min(max(row0 + row, lo), hi - 1);
+            r[i] = *reinterpret_cast<const typename Ops<T>::Frag*>(base + at * row_stride + (c < dim ? c : 0));
+        }
+    }
+    __device__ __forceinline__ void store(T* tile, int dim) const {
+        constexpr int kPitch = pitch<T, DP>();
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, c = (idx - row * kChunks) * Ops<T>::W;
+            *reinterpret_cast<typename Ops<T>::Frag*>(tile + row * kPitch + c) = c < dim ? r[i] : typename Ops<T>::Frag{};
+        }
+    }
+};
+
+// ---- scores ------------------------------------------------------------------------------------------------------------
+// From q.k to log2(e) u: with a cap, cap log2(e) tanh(scale q.k / cap).
+struct Score {
+    float mul, cap, inv;                 // inv: 1 / (cap log2 e), turns the result back into the tanh
+    bool capped;
+
+    __device__ __forceinline__ Score(const Dev& a) {
+        capped = a.softcap > 0.f;
+        cap = a.softcap * kLog2e;
+        inv = capped ? 1.f / cap : 0.f;
+        mul = capped ? a.scale / a.softcap : a.scale * kLog2e;
+    }
+    template <typename T>
+    __device__ __forceinline__ void apply(f32x16& s) const {
+        if (!capped) {
+            s *= mul;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = s[r] * mul;
+                if constexpr (__is_same(T, float)) {
+                    s[r] = cap * tanhf(x);
+                } else {
+                    // tanh x = 1 - 2 / (e^2x + 1): off by some 2^-23 of the cap, far below the rounding of 16-bit weights
+                    const float e = exp2_(x * (2.f * kLog2e));
+                    s[r] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(e + 1.f), cap);
+                }
+            }
+        }
+    }
+    // d u / d t
+    __device__ __forceinline__ float slope(float u) const {
+        const float t = u * inv;
+        return fmaf(-t, t, 1.f);
+    }
+};
+
+// tile row of register r of this lane half
+__device__ __forceinline__ int reg_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+bool check_args(const ddpm_span_attention_args& a);              // span_attention_fwd.hip
+Dev dev_args(const ddpm_span_attention_args& a);
+
+// f(head size as a compile-time constant): dim rounded up to a multiple of 32
+template <typename F>
+void for_dim(int dim, F&& f) {
+    if (dim <= 32)
+        f(std::integral_constant<int, 32>{});
+    else if (dim <= 64)
+        f(std::integral_constant<int, 64>{});
+    else if (dim <= 96)
+        f(std::integral_constant<int, 96>{});
+    else
+        f(std::integral_constant<int, 128>{});
+}
+
+}  // namespace span

@@ -1,0 +1,405 @@
+// Span attention, gradient (the mathematics and the two products are in span_attention.h):
+//   D_i = sum_c dout_ic out_ic,  p_ij = exp(w_ij - lse_i),  dp_ij = dout_i . v_j,  ds_ij = scale (du/dt)_ij p_ij (dp_ij - D_i)
+//   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
+// in two kernels, each of which recomputes the scores: dq walks over keys with rows in registers, dk and dv over rows with keys in
+// registers. That is 7 products for the 5 of a single kernel, whose dq would be added up with atomics in an order that changes
+// from call to call, and in fp32 memory that must be cleared before and converted behind. The gradient of a key/value head is
+// summed over the query heads that share it inside its workgroup.
+#include "span_attention.h"
+
+using ddpm::as_stream;
+
+namespace {
+
+using namespace span;
+
+constexpr int kRows = 128;               // rows (dq) or keys (dk, dv) of a workgroup, 32 a wave
+
+// What 32 rows see together: keys [lo, hi) are seen by some of them, [all_lo, all_hi) by all (all_lo = INT_MAX when one sees none).
+struct Seen {
+    int lo, hi, all_lo, all_hi;
+};
+
+struct Work {
+    float* delta;                        // D: [batch][heads][nq]
+    Seen* seen;                          // [batch][groups], groups of 32 rows
+    float* largest;                      // fp16: largest |ds| of the rows of a group: [batch][heads][groups]
+    int groups;
+};
+
+// fp16 has five bits of exponent, and score gradients are as small as a loss makes them: they are scaled by a power of two
+// that brings the largest to 2^13 ... 2^14 before they are rounded, and the sums are scaled back. Limits keep both factors finite.
+__device__ __forceinline__ float gain_for(float largest) {
+    int e = static_cast<int>((__builtin_bit_cast(unsigned, largest) >> 23) & 255) - 127;
+    e = max(-100, min(100, 13 - e));
+    return __builtin_bit_cast(float, static_cast<unsigned>(127 + e) << 23);
+}
+__device__ __forceinline__ float inverse_gain(float gain) {
+    return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(unsigned, gain));
+}
+
+// lse in units of log 2, such that exp2(score - it) is nought for a row whose weights are all nought
+__device__ __forceinline__ float stat_of(float lse) { return lse == -INFINITY ? -kNoMax : lse * kLog2e; }
+
+template <typename T, int DP>
+__device__ __forceinline__ void write_row(T* out, const f32x16* acc, float f, int dim) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * db + 8 * g + 4 * half;
+            T4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[db][4 * g + e] * f);
+            if (d < dim) *reinterpret_cast<T4*>(out + d) = o;
+        }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_kernel(const Dev a, const Work work) {
+    constexpr int kPitch = pitch<T, DP>(), kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+    constexpr bool kGain = __is_same(T, _Float16);
+    __shared__ __attribute__((aligned(16))) T k_tile[kTile * kPitch];
+    __shared__ __attribute__((aligned(16))) T v_tile[kTile * kPitch];
+    __shared__ int bounds[2][4];
+
+    const dim3 id = ddpm::xcd_block();
+    const int block = gridDim.x - 1 - id.x, head = id.y, b = id.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int i = block * kRows + wave * 32 + (lane & 31);
+    const bool real = i < a.nq;
+    const int kv = head / a.group;
+    const Row row = real ? row_of(a, b, i) : no_row();
+    int wlo = row.lo, whi = row.hi;
+    join_rows(wlo, whi);
+    if (head == 0) {
+        int alo = row.lo, ahi = row.hi;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            alo = max(alo, __shfl_xor(alo, d));
+            ahi = min(ahi, __shfl_xor(ahi, d));
+        }
+        if (lane == 0) work.seen[static_cast<int64_t>(b) * work.groups + block * 4 + wave] = {wlo, whi, alo, ahi};
+    }
+    if (lane == 0) {
+        bounds[0][wave] = wlo;
+        bounds[1][wave] = whi;
+    }
+    const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
+    OwnRow<T, DP> q, dout;
+    q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
+    dout.load(real ? static_cast<const T*>(a.dout) + b * a.sdo.batch + i * a.sdo.row + head * a.sdo.head : nullptr, a.dim);
+    float delta = 0.f, stat = -kNoMax;
+    {
+        OwnRow<T, DP> out;
+        out.load(real ? static_cast<const T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head : nullptr, a.dim);
+#pragma unroll
+        for (int s = 0; s < OwnRow<T, DP>::kSteps; ++s)
+#pragma unroll
+            for (int e = 0; e < Ops<T>::W; ++e) delta = fmaf(static_cast<float>(dout.f[s][e]), static_cast<float>(out.f[s][e]), delta);
+        delta += other_half(delta);
+    }
+    if (real) {
+        stat = stat_of(a.lse[at]);
+        if (half == 0) work.delta[at] = delta;
+    }
+    __syncthreads();
+    const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
+    const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    const int first = lo < hi ? lo / kTile : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;
+
+    const Score score(a);
+    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    const T* k = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
+    const T* v = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
+    f32x16 acc[DP / 32] = {};
+    float gain = gain_for(0.f), largest = 0.f;
+    Staged<T, DP> ks, vs;
+    if (first < last) {
+        ks.load(k, a.sk.row, first * kTile, lo, hi, a.dim);
+        vs.load(v, a.sv.row, first * kTile, lo, hi, a.dim);
+    }
+    for (int t = first; t < last; ++t) {
+        __syncthreads();
+        ks.store(k_tile, a.dim);
+        vs.store(v_tile, a.dim);
+        __syncthreads();
+        const int j0 = t * kTile;
+        if (t + 1 < last) {
+            ks.load(k, a.sk.row, j0 + kTile, lo, hi, a.dim);
+            vs.load(v, a.sv.row, j0 + kTile, lo, hi, a.dim);
+        }
+        if (j0 + kTile <= wlo || j0 >= whi) continue;
+        const bool whole = __all(row.lo <= j0 && row.hi >= j0 + kTile);
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; ++kb) {
+            f32x16 s = q.template dot<kPitch>(k_tile + kb * 32 * kPitch);
+            const f32x16 dp = dout.template dot<kPitch>(v_tile + kb * 32 * kPitch);
+            score.apply<T>(s);
+            f32x16 ds;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = j0 + 32 * kb + reg_row(e, half);
+                float w = s[e];
+                if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(row.pos - j)), w);
+                float d = exp2_(w - stat) * (dp[e] - delta) * a.scale;
+                if (score.capped) d *= score.slope(s[e]);
+                if (!whole && (j < row.lo || j >= row.hi)) d = 0.f;
+                ds[e] = d;
+            }
+            if constexpr (kGain) {
+                float m = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(ds[e]));
+                m = fmaxf(m, other_half(m));
+                largest = fmaxf(largest, m);
+                if (__any(m * gain >= 32768.f)) {
+                    const float next = fminf(gain, gain_for(m)), f = next * inverse_gain(gain);
+                    gain = next;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) acc[db] *= f;
+                }
+                ds *= gain;
+            }
+            Ops<T>::template spread<DP, kPitch>(acc, k_tile + kb * 32 * kPitch, Ops<T>::pack(ds));
+        }
+    }
+    if constexpr (kGain) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+        if (lane == 0) work.largest[(static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave] = largest;
+    }
+    if (real)
+        write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, kGain ? inverse_gain(gain) : 1.f, a.dim);
+}
+
+// The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other.
+template <int GROUPS>                    // groups of 32 rows in a tile
+struct Tiles {
+    const Seen* seen;
+    int groups, tiles, heads, begin, end;
+    int head, base;                      // 64 tiles from `base` on are in `mask`
+    unsigned long long mask;
+
+    __device__ __forceinline__ void look() {
+        const int t = base + (threadIdx.x & 63);
+        bool any = false;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+            if (t * GROUPS + g < groups) {
+                const Seen s = seen[t * GROUPS + g];
+                any |= s.lo < end && s.hi > begin;
+            }
+        mask = __ballot(any);
+    }
+    // moves to the next tile; false behind the last one
+    __device__ __forceinline__ bool next(int& h, int& tile) {
+        while (mask == 0) {
+            base += 64;
+            if (base >= tiles) {
+                base = 0;
+                if (++head >= heads) return false;
+            }
+            look();
+        }
+        tile = base + __builtin_ctzll(mask);
+        mask &= mask - 1;
+        h = head;
+        return true;
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const Dev a, const Work work) {
+    constexpr int kPitch = pitch<T, DP>(), kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+    constexpr bool kGain = __is_same(T, _Float16);
+    constexpr float kUnshift = 1.f / (1 << Ops<T>::kShift);
+    __shared__ __attribute__((aligned(16))) T q_tile[kTile * kPitch];
+    __shared__ __attribute__((aligned(16))) T do_tile[kTile * kPitch];
+    __shared__ __attribute__((aligned(16))) float stat_tile[kTile], delta_tile[kTile];
+    __shared__ __attribute__((aligned(16))) int lo_tile[kTile], hi_tile[kTile], pos_tile[kTile];
+    __shared__ float wave_max[4];
+
+    const dim3 id = ddpm::xcd_block();
+    const int kv = id.y, b = id.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int begin = id.x * kRows, w0 = begin + wave * 32, j = w0 + (lane & 31);   // keys of the workgroup, the wave, the lane
+    const bool real = j < a.nk;
+    OwnRow<T, DP> k, v;
+    k.load(real ? static_cast<const T*>(a.k) + b * a.sk.batch + j * a.sk.row + kv * a.sk.head : nullptr, a.dim);
+    v.load(real ? static_cast<const T*>(a.v) + b * a.sv.batch + j * a.sv.row + kv * a.sv.head : nullptr, a.dim);
+
+    float gain = 1.f;
+    if constexpr (kGain) {
+        const float* largest = work.largest + (static_cast<int64_t>(b) * a.heads + kv * a.group) * work.groups;
+        float m = 0.f;
+        for (int64_t x = threadIdx.x; x < static_cast<int64_t>(a.group) * work.groups; x += kThreads) m = fmaxf(m, largest[x]);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        if (lane == 0) wave_max[wave] = m;
+        __syncthreads();
+        gain = gain_for(fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3])));
+    }
+
+    const Score score(a);
+    f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+    Tiles<kBlocks> tiles;
+    tiles.seen = work.seen + static_cast<int64_t>(b) * work.groups;
+    tiles.groups = work.groups;
+    tiles.tiles = (a.nq + kTile - 1) / kTile;
+    tiles.heads = a.group;
+    tiles.begin = begin;
+    tiles.end = min(begin + kRows, a.nk);
+    tiles.head = tiles.base = 0;
+    tiles.look();
+
+    Staged<T, DP> qs, dos;
+    Row row = no_row();
+    float stat = 0.f, delta = 0.f;
+    bool dead[Staged<T, DP>::kLoads];    // rows that see nothing: what q and dout hold there is not looked at
+    const auto load = [&](int h, int tile) {
+        const int head = kv * a.group + h, i0 = tile * kTile;
+        qs.load(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, a.sq.row, i0, 0, a.nq, a.dim);
+        dos.load(static_cast<const T*>(a.dout) + b * a.sdo.batch + head * a.sdo.head, a.sdo.row, i0, 0, a.nq, a.dim);
+        bool all = true;
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g)
+            if (tile * kBlocks + g < work.groups) all &= tiles.seen[tile * kBlocks + g].all_lo != INT32_MAX;
+#pragma unroll
+        for (int x = 0; x < Staged<T, DP>::kLoads; ++x) {
+            dead[x] = false;
+            if (!all) {
+                const int i = i0 + (x * kThreads + static_cast<int>(threadIdx.x)) / Staged<T, DP>::kChunks;
+                dead[x] = i >= a.nq || row_of(a, b, i).hi == 0;
+            }
+        }
+        if (threadIdx.x < kTile) {
+            const int i = i0 + threadIdx.x;
+            row = no_row();
+            stat = -kNoMax;
+            delta = 0.f;
+            if (i < a.nq) {
+                const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
+                row = row_of(a, b, i);
+                stat = stat_of(a.lse[at]);
+                delta = work.delta[at];
+            }
+        }
+    };
+
+    int h = 0, tile = 0;
+    bool more = tiles.next(h, tile);
+    if (more) load(h, tile);
+    while (more) {
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < Staged<T, DP>::kLoads; ++x)
+            if (dead[x]) qs.r[x] = dos.r[x] = typename Ops<T>::Frag{};
+        qs.store(q_tile, a.dim);
+        dos.store(do_tile, a.dim);
+        if (threadIdx.x < kTile) {
+            lo_tile[threadIdx.x] = row.lo;
+            hi_tile[threadIdx.x] = row.hi;
+            pos_tile[threadIdx.x] = row.pos;
+            stat_tile[threadIdx.x] = stat;
+            delta_tile[threadIdx.x] = delta;
+        }
+        __syncthreads();
+        const int now = tile, head = kv * a.group + h;
+        more = tiles.next(h, tile);
+        if (more) load(h, tile);
+        const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g) {
+            if (now * kBlocks + g >= work.groups) continue;
+            const Seen seen = tiles.seen[now * kBlocks + g];
+            if (seen.lo >= w0 + 32 || seen.hi <= w0) continue;
+            const bool whole = seen.all_lo <= w0 && seen.all_hi >= w0 + 32;
+            f32x16 s = k.template dot<kPitch>(q_tile + g * 32 * kPitch);
+            const f32x16 dp = v.template dot<kPitch>(do_tile + g * 32 * kPitch);
+            score.apply<T>(s);
+            f32x16 p, ds;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int at = 32 * g + 8 * x + 4 * half;              // four rows
+                const f32x4 stats = *reinterpret_cast<const f32x4*>(stat_tile + at);
+                const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float w = s[4 * x + e] + Ops<T>::kShift - stats[e];
+                    if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(pos_tile[at + e] - j)), w);
+                    float y = exp2_(w), d = y * (dp[4 * x + e] - deltas[e]) * (a.scale * kUnshift);
+                    if (score.capped) d *= score.slope(s[4 * x + e]);
+                    if (!whole && (j < lo_tile[at + e] || j >= hi_tile[at + e])) y = d = 0.f;
+                    p[4 * x + e] = y;
+                    ds[4 * x + e] = kGain ? d * gain : d;
+                }
+            }
+            Ops<T>::template spread<DP, kPitch>(dv, do_tile + g * 32 * kPitch, Ops<T>::pack(p));
+            Ops<T>::template spread<DP, kPitch>(dk, q_tile + g * 32 * kPitch, Ops<T>::pack(ds));
+        }
+    }
+    if (!real) return;
+    write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, kGain ? inverse_gain(gain) : 1.f, a.dim);
+    write_row<T, DP>(static_cast<T*>(a.dv) + b * a.sdv.batch + j * a.sdv.row + kv * a.sdv.head, dv, kUnshift, a.dim);
+}
+
+int groups_of(int nq) { return (nq + kRows - 1) / kRows * 4; }
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+template <typename T>
+void launch(const ddpm_span_attention_args& a, void* workspace, hipStream_t stream) {
+    const Dev d = dev_args(a);
+    Work work = {};
+    work.groups = groups_of(a.nq);
+    char* at = static_cast<char*>(workspace);
+    work.seen = reinterpret_cast<Seen*>(at);
+    at += static_cast<int64_t>(a.batch) * work.groups * sizeof(Seen);
+    work.delta = reinterpret_cast<float*>(at);
+    at += round16(static_cast<int64_t>(a.batch) * a.heads * a.nq * 4);
+    work.largest = reinterpret_cast<float*>(at);
+    for_dim(a.dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        if (a.nq > 0) dq_kernel<T, DP><<<dim3(work.groups / 4, a.heads, a.batch), kThreads, 0, stream>>>(d, work);
+        if (a.nk > 0) dkv_kernel<T, DP><<<dim3((a.nk + kRows - 1) / kRows, a.kv_heads, a.batch), kThreads, 0, stream>>>(d, work);
+    });
+}
+
+bool check_bwd(const ddpm_span_attention_args& a) {
+    if (!check_args(a)) return false;
+    const int w = a.type == DDPM_F32 ? 4 : 8;
+    for (const int64_t* s : {a.dout_stride, a.dq_stride, a.dk_stride, a.dv_stride})
+        if (s[0] % w || s[1] % w || s[2] % w) return false;
+    return true;
+}
+
+}  // namespace
+
+extern "C" int64_t ddpm_span_attention_bwd_workspace(const ddpm_span_attention_args* a) {
+    if (!a || !check_bwd(*a)) return ddpm::fail_invalid("span attention sizes, type or strides");
+    const int64_t groups = groups_of(a->nq);
+    return static_cast<int64_t>(a->batch) * groups * static_cast<int64_t>(sizeof(Seen)) +
+           round16(static_cast<int64_t>(a->batch) * a->heads * a->nq * 4) +
+           (a->type == DDPM_F16 ? round16(static_cast<int64_t>(a->batch) * a->heads * groups * 4) : 0);
+}
+
+extern "C" int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* workspace, void* stream) {
+    DDPM_REQUIRE(a && check_bwd(*a));
+    if (a->batch == 0) return DDPM_OK;
+    DDPM_REQUIRE(a->nq == 0 || (a->q && a->out && a->lse && a->dout && a->dq));
+    DDPM_REQUIRE(a->nk == 0 || (a->k && a->v && a->dk && a->dv));
+    for (const void* p : {a->q, a->k, a->v, static_cast<const void*>(a->out), a->dout, static_cast<const void*>(a->dq),
+                          static_cast<const void*>(a->dk), static_cast<const void*>(a->dv), static_cast<const void*>(workspace)})
+        DDPM_REQUIRE(ddpm::aligned16(p));
+    DDPM_REQUIRE(a->nq == 0 || workspace);
+    if (a->type == DDPM_F32)
+        launch<float>(*a, workspace, as_stream(stream));
+    else if (a->type == DDPM_BF16)
+        launch<__bf16>(*a, workspace, as_stream(stream));
+    else
+        launch<_Float16>(*a, workspace, as_stream(stream));
+    return ddpm::check_launch("span attention backward");
+}

@@ -1,0 +1,314 @@
+// Span attention, forward (the mathematics and the two products are in span_attention.h).
+//
+// A workgroup of 4 waves takes 128 rows of one head, 32 a wave, and walks over the keys that any of them sees, a tile of 64
+// (fp32: 32) at a time: k and v go through registers into LDS, the next tile's loads fly while this one is worked on, and a
+// running maximum and sum turn the scores into weights in one pass. With few rows (single tokens) the query heads that share
+// a key/value head are rows of one workgroup, and the keys are split over workgroups whose parts a second kernel joins.
+#include <algorithm>
+
+#include "span_attention.h"
+
+using ddpm::as_stream;
+
+namespace span {
+
+bool check_args(const ddpm_span_attention_args& a) {
+    const int w = a.type == DDPM_F32 ? 4 : 8;
+    const auto fits = [&](const int64_t* s) { return s[0] % w == 0 && s[1] % w == 0 && s[2] % w == 0; };
+    return (a.type == DDPM_F32 || a.type == DDPM_BF16 || a.type == DDPM_F16) && a.batch >= 0 && a.batch <= 65535 && a.nq >= 0 && a.nk >= 0 &&
+           a.heads >= 1 && a.heads <= 65535 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0 && a.dim >= w &&
+           a.dim <= DDPM_SPAN_ATTENTION_MAX_DIM && a.dim % w == 0 && a.nq <= (1 << 30) && a.nk <= (1 << 30) && a.softcap >= 0.f &&
+           a.softcap <= 1e30f && a.scale >= -1e30f && a.scale <= 1e30f && fits(a.q_stride) && fits(a.k_stride) && fits(a.v_stride) &&
+           fits(a.out_stride);
+}
+
+Dev dev_args(const ddpm_span_attention_args& a) {
+    const auto strides = [](const int64_t* s) { return Strides{s[0], s[1], s[2]}; };
+    Dev d = {};
+    d.nq = a.nq;
+    d.nk = a.nk;
+    d.heads = a.heads;
+    d.group = a.heads / a.kv_heads;
+    d.dim = a.dim;
+    d.causal = a.causal != 0;
+    d.scale = a.scale;
+    d.softcap = a.softcap;
+    d.slopes = a.slopes;
+    d.spans = a.spans;
+    d.positions = a.positions;
+    d.span_batch = a.span_batch_stride;
+    d.position_batch = a.position_batch_stride;
+    d.q = a.q;
+    d.k = a.k;
+    d.v = a.v;
+    d.out = a.out;
+    d.lse = a.lse;
+    d.sq = strides(a.q_stride);
+    d.sk = strides(a.k_stride);
+    d.sv = strides(a.v_stride);
+    d.so = strides(a.out_stride);
+    d.dout = a.dout;
+    d.dq = a.dq;
+    d.dk = a.dk;
+    d.dv = a.dv;
+    d.sdo = strides(a.dout_stride);
+    d.sdq = strides(a.dq_stride);
+    d.sdk = strides(a.dk_stride);
+    d.sdv = strides(a.dv_stride);
+    return d;
+}
+
+}  // namespace span
+
+namespace {
+
+using namespace span;
+
+constexpr int kRows = 128;               // rows of a workgroup
+
+// How the rows and keys of a call are spread over workgroups.
+struct Plan {
+    int pack;                            // query heads that are rows of one workgroup
+    int blocks;                          // workgroups along the rows
+    int splits;                          // parts of the keys
+};
+
+Plan plan_of(const ddpm_span_attention_args& a) {
+    Plan p;
+    const int group = a.heads / a.kv_heads, tile = a.type == DDPM_F32 ? 32 : 64;
+    // Rows of one head that do not fill a workgroup share it with the other heads of their group: k and v are read once for all.
+    p.pack = a.nq < kRows ? group : 1;
+    p.blocks = static_cast<int>((static_cast<int64_t>(a.nq) * p.pack + kRows - 1) / kRows);
+    const int64_t all = static_cast<int64_t>(p.blocks) * (a.heads / p.pack) * a.batch, tiles = (a.nk + tile - 1) / tile;
+    // Two workgroups a compute unit, each with 4 tiles at least, so that joining stays small beside reading.
+    p.splits = all > 0 && all < 512 ? static_cast<int>(std::min<int64_t>((512 + all - 1) / all, tiles / 4)) : 1;
+    p.splits = std::max(1, std::min(p.splits, 128));
+    return p;
+}
+
+struct Parts {                           // of a split call: per part and row the sum before division, its maximum and weight sum
+    float* out;                          // [splits][batch][heads][nq][dim]
+    float* stat;                         // [splits][batch][heads][nq][2]
+    int splits;
+    int64_t rows;                        // batch * heads * nq
+};
+
+template <typename T, int DP, bool SPLIT>
+__global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int pack, const Parts parts) {
+    constexpr int kPitch = pitch<T, DP>(), kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+    __shared__ __attribute__((aligned(16))) T k_tile[kTile * kPitch];
+    __shared__ __attribute__((aligned(16))) T v_tile[kTile * kPitch];
+    __shared__ int bounds[2][4];
+
+    // x: row blocks (the last first: under causal order they have most to do), and with SPLIT the parts of the keys beside them
+    const dim3 id = ddpm::xcd_block();
+    const int part = SPLIT ? id.x % parts.splits : 0;
+    const int block = SPLIT ? id.x / parts.splits : gridDim.x - 1 - id.x;
+    const int b = id.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int r = block * kRows + wave * 32 + (lane & 31);          // row of this lane's column
+    const bool real = r < a.nq * pack;
+    const int i = real ? r / pack : 0;
+    const int head = id.y * pack + (real ? r % pack : 0);
+    const int kv = (id.y * pack) / a.group;
+
+    const Row row = real ? row_of(a, b, i) : no_row();
+    int wlo = row.lo, whi = row.hi;
+    join_rows(wlo, whi);
+    if (lane == 0) {
+        bounds[0][wave] = wlo;
+        bounds[1][wave] = whi;
+    }
+    OwnRow<T, DP> q;
+    q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
+    __syncthreads();
+    const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
+    const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+
+    int first = lo < hi ? lo / kTile : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;   // tiles
+    if (SPLIT) {
+        const int n = last - first, begin = first;
+        first = begin + static_cast<int>(static_cast<int64_t>(n) * part / parts.splits);
+        last = begin + static_cast<int>(static_cast<int64_t>(n) * (part + 1) / parts.splits);
+    }
+
+    const Score score(a);
+    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    const T* k = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
+    const T* v = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
+
+    f32x16 acc[DP / 32] = {};
+    float top = kNoMax, sum = 0.f;       // of this column: maximum of all its scores, sum of this lane half's weights
+    Staged<T, DP> ks, vs;
+    if (first < last) {
+        ks.load(k, a.sk.row, first * kTile, lo, hi, a.dim);
+        vs.load(v, a.sv.row, first * kTile, lo, hi, a.dim);
+    }
+    for (int t = first; t < last; ++t) {
+        __syncthreads();
+        ks.store(k_tile, a.dim);
+        vs.store(v_tile, a.dim);
+        __syncthreads();
+        const int j0 = t * kTile;
+        if (t + 1 < last) {
+            ks.load(k, a.sk.row, j0 + kTile, lo, hi, a.dim);
+            vs.load(v, a.sv.row, j0 + kTile, lo, hi, a.dim);
+        }
+        if (j0 + kTile <= wlo || j0 >= whi) continue;               // nothing here for this wave's rows
+        f32x16 s[kBlocks];
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; ++kb) {
+            s[kb] = q.template dot<kPitch>(k_tile + kb * 32 * kPitch);
+            score.apply<T>(s[kb]);
+        }
+        if (a.slopes) {
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[kb][e] = fmaf(-slope, fabsf(static_cast<float>(row.pos - (j0 + 32 * kb + reg_row(e, half)))), s[kb][e]);
+        }
+        if (!__all(row.lo <= j0 && row.hi >= j0 + kTile)) {
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = j0 + 32 * kb + reg_row(e, half);
+                    if (j < row.lo || j >= row.hi) s[kb][e] = -INFINITY;
+                }
+        }
+        float m = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, s[kb][e]);
+        m = fmaxf(m, other_half(m));
+        if (__any(m > top)) {
+            m = fmaxf(m, top);
+            const float f = exp2_(top - m);
+            top = m;
+            sum *= f;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) acc[db] *= f;
+        }
+        const float shift = Ops<T>::kShift - top;
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[kb][e] = exp2_(s[kb][e] + shift);
+                sum += s[kb][e];
+            }
+            Ops<T>::template spread<DP, kPitch>(acc, v_tile + kb * 32 * kPitch, Ops<T>::pack(s[kb]));
+        }
+    }
+
+    sum += other_half(sum);
+    if (!real) return;
+    const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
+    if (SPLIT) {
+        float* out = parts.out + (part * parts.rows + at) * a.dim;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * db + 8 * g + 4 * half;
+                if (d < a.dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+            }
+        if (half == 0) {
+            parts.stat[2 * (part * parts.rows + at)] = top - Ops<T>::kShift;
+            parts.stat[2 * (part * parts.rows + at) + 1] = sum;
+        }
+        return;
+    }
+    if (a.lse && half == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top - Ops<T>::kShift + log2f(sum)) * kLn2;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = static_cast<T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * db + 8 * g + 4 * half;
+            T4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[db][4 * g + e] * inv);
+            if (d < a.dim) *reinterpret_cast<T4*>(out + d) = o;
+        }
+}
+
+// Joins the parts of a split call: a wave per row, 4 channels a lane (lanes behind dim idle).
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const Dev a, const Parts parts) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (at >= parts.rows) return;
+    float top = kNoMax;
+    for (int p = 0; p < parts.splits; ++p) top = fmaxf(top, parts.stat[2 * (p * parts.rows + at)]);
+    float sum = 0.f;
+    f32x4 acc = {};
+    for (int p = 0; p < parts.splits; ++p) {
+        const float f = exp2_(parts.stat[2 * (p * parts.rows + at)] - top);
+        sum = fmaf(parts.stat[2 * (p * parts.rows + at) + 1], f, sum);
+        if (4 * lane < a.dim) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(parts.out + (p * parts.rows + at) * a.dim + 4 * lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(x[e], f, acc[e]);
+        }
+    }
+    const int i = static_cast<int>(at % a.nq);
+    const int64_t bh = at / a.nq;
+    const int head = static_cast<int>(bh % a.heads);
+    const int64_t b = bh / a.heads;
+    if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    if (4 * lane >= a.dim) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[e] * inv);
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head + 4 * lane) = o;
+}
+
+template <typename T>
+void launch(const ddpm_span_attention_args& a, const Plan& plan, void* workspace, hipStream_t stream) {
+    const Dev d = dev_args(a);
+    Parts parts = {};
+    parts.splits = plan.splits;
+    parts.rows = static_cast<int64_t>(a.batch) * a.heads * a.nq;
+    parts.out = static_cast<float*>(workspace);
+    parts.stat = parts.out + parts.splits * parts.rows * a.dim;
+    const dim3 grid(plan.blocks * plan.splits, a.heads / plan.pack, a.batch);
+    for_dim(a.dim, [&](auto dp) {
+        if (plan.splits > 1)
+            fwd_kernel<T, decltype(dp)::value, true><<<grid, kThreads, 0, stream>>>(d, plan.pack, parts);
+        else
+            fwd_kernel<T, decltype(dp)::value, false><<<grid, kThreads, 0, stream>>>(d, plan.pack, parts);
+    });
+    if (plan.splits > 1) join_kernel<T><<<static_cast<unsigned>((parts.rows + 3) / 4), 256, 0, stream>>>(d, parts);
+}
+
+}  // namespace
+
+extern "C" int64_t ddpm_span_attention_fwd_workspace(const ddpm_span_attention_args* a) {
+    if (!a || !span::check_args(*a)) return ddpm::fail_invalid("span attention sizes, type or strides");
+    if (a->batch == 0 || a->nq == 0) return 0;
+    const Plan plan = plan_of(*a);
+    return plan.splits == 1 ? 0 : static_cast<int64_t>(plan.splits) * a->batch * a->heads * a->nq * (a->dim + 2) * 4;
+}
+
+extern "C" int ddpm_span_attention_fwd(const ddpm_span_attention_args* a, void* workspace, void* stream) {
+    DDPM_REQUIRE(a && span::check_args(*a));
+    if (a->batch == 0 || a->nq == 0) return DDPM_OK;
+    DDPM_REQUIRE(a->q && a->out && (a->nk == 0 || (a->k && a->v)));
+    DDPM_REQUIRE(ddpm::aligned16(a->q) && ddpm::aligned16(a->k) && ddpm::aligned16(a->v) && ddpm::aligned16(a->out));
+    const Plan plan = plan_of(*a);
+    DDPM_REQUIRE(plan.splits == 1 || (workspace && ddpm::aligned16(workspace)));
+    if (a->type == DDPM_F32)
+        launch<float>(*a, plan, workspace, as_stream(stream));
+    else if (a->type == DDPM_BF16)
+        launch<__bf16>(*a, plan, workspace, as_stream(stream));
+    else
+        launch<_Float16>(*a, plan, workspace, as_stream(stream));
+    return ddpm::check_launch("span attention forward");
+}

@@ -409,6 +409,51 @@ int ddpm_self_attention_infer(const float* x, int ldx, const float* wqkv_packed,
                               int batch, int n, int c, int dq, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Span attention: several heads (key/value heads may be shared by groups of query heads), scores capped by a tanh, a bias
+ * by distance, and masks in which every row sees one span of keys -- documents packed into a sequence, prefixes, padded
+ * lengths, windows, causal order. For rows i (queries) and keys j of one head h, with g = h / (heads / kv_heads):
+ *   t = scale * q_i . k_j        u = softcap * tanh(t / softcap)   (u = t when softcap is 0)
+ *   w = u - slopes[h] * |position_i - j|      for the keys that row i sees, first_i <= j < last_i (and j <= position_i when causal)
+ *   out_i = sum_j softmax_j(w) v_j            lse_i = log sum_j exp(w)
+ * A row that sees no key (or whose keys all have weight nought) has out = 0, lse = -infinity and no gradient. Keys that no
+ * row sees have gradient 0, and what q, k and v hold there does not matter; a value that is not finite at a key that some row sees
+ * may reach other rows of that batch entry, as a product with weight nought does.
+ * Element (b, n, h, c) of a tensor lies at its base + b*stride[0] + n*stride[1] + h*stride[2] + c. Bases must be 16-byte
+ * aligned, and dim and the strides of q, k, v, out and the gradients multiples of 16 bytes (4 fp32, 8 16-bit elements).
+ * Arithmetic: fp32 inputs use the fp32 matrix instructions; 16-bit inputs have their weights and score gradients rounded
+ * to 16 bits before the second product; scores, softmax statistics and sums are fp32 throughout.
+ * Stands beside ddpm_attention_fwd / _bwd (one head, no mask, second-iteration/unet.py:50-61).
+ * ------------------------------------------------------------------------------------- */
+#define DDPM_SPAN_ATTENTION_MAX_DIM 128
+typedef struct ddpm_span_attention_args {
+    int32_t type;                    /* DDPM_F32, BF16, F16: of q, k, v, out and the gradients */
+    int32_t batch, nq, nk, heads, kv_heads, dim;   /* heads a multiple of kv_heads, dim <= DDPM_SPAN_ATTENTION_MAX_DIM */
+    int32_t causal;
+    float scale, softcap;            /* softcap >= 0 */
+    const float* slopes;             /* [heads] or NULL */
+    const int32_t* spans;            /* [batch or 1][nq][2]: first key, last key + 1; cut to [0, nk). NULL: all keys */
+    const int32_t* positions;        /* [batch or 1][nq]; NULL: row i stands at i + nk - nq */
+    int64_t span_batch_stride, position_batch_stride;   /* elements; 0 = shared by the batch */
+    const void *q, *k, *v;
+    void* out;
+    float* lse;                      /* [batch][heads][nq]; forward: may be NULL */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* elements: batch, row, head */
+    /* the backward call; out and lse are the forward's */
+    const void* dout;
+    void *dq, *dk, *dv;
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} ddpm_span_attention_args;
+
+/* Bytes of workspace (16-byte aligned, contents unspecified afterwards) of the two calls; negative for bad arguments.
+ * Depends on the sizes and the type alone. The forward call needs one when few rows meet many keys: the keys are then
+ * split over workgroups and the parts joined. */
+int64_t ddpm_span_attention_fwd_workspace(const ddpm_span_attention_args* a);
+int64_t ddpm_span_attention_bwd_workspace(const ddpm_span_attention_args* a);
+int ddpm_span_attention_fwd(const ddpm_span_attention_args* a, void* workspace, void* stream);
+/* dq, dk and dv are written whole; the same inputs give the same bits (no atomics). */
+int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* workspace, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Train-mode BatchNorm2d (+ activation / residual / time-embedding add), forward and backward.
  * Replaces nn.BatchNorm2d in training mode together with the ReLU/GELU, the residual add of
  * ResidualBlock and the `+ time_emb` that follow it: first-iteration/unet.py:17-21,
