@@ -118,11 +118,14 @@ class _SpanAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse, slopes, spans, positions)
         ctx.how = scale, softcap, causal
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 9
         q, k, v, out, lse, slopes, spans, positions = ctx.saved_tensors
         scale, softcap, causal = ctx.how
         dout = _fit(dout, _TYPES[q.dtype][1])

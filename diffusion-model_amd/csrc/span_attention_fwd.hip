@@ -65,6 +65,7 @@ namespace {
 using namespace span;
 
 constexpr int kRows = 128;               // rows of a workgroup
+constexpr int kMaxSplits = 128;          // parts of the keys
 
 // How the rows and keys of a call are spread over workgroups.
 struct Plan {
@@ -82,7 +83,7 @@ Plan plan_of(const ddpm_span_attention_args& a) {
     const int64_t all = static_cast<int64_t>(p.blocks) * (a.heads / p.pack) * a.batch, tiles = (a.nk + tile - 1) / tile;
     // Two workgroups a compute unit, each with 4 tiles at least, so that joining stays small beside reading.
     p.splits = all > 0 && all < 512 ? static_cast<int>(std::min<int64_t>((512 + all - 1) / all, tiles / 4)) : 1;
-    p.splits = std::max(1, std::min(p.splits, 128));
+    p.splits = std::max(1, std::min(p.splits, kMaxSplits));
     return p;
 }
 
@@ -237,37 +238,63 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         }
 }
 
-// Joins the parts of a split call: a wave per row, 4 channels a lane (lanes behind dim idle).
+// Joins the parts of a split call, a workgroup per row: the parts' maxima and sums at once, then 8 groups of 32 lanes add up every
+// eighth part, 4 channels a lane (lanes behind dim idle), and the groups are added in order. 128 parts of 32 rows take 5 us; a
+// wave per row that walked over the parts took 95.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const Dev a, const Parts parts) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (at >= parts.rows) return;
-    float top = kNoMax;
-    for (int p = 0; p < parts.splits; ++p) top = fmaxf(top, parts.stat[2 * (p * parts.rows + at)]);
-    float sum = 0.f;
-    f32x4 acc = {};
-    for (int p = 0; p < parts.splits; ++p) {
-        const float f = exp2_(parts.stat[2 * (p * parts.rows + at)] - top);
-        sum = fmaf(parts.stat[2 * (p * parts.rows + at) + 1], f, sum);
-        if (4 * lane < a.dim) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(parts.out + (p * parts.rows + at) * a.dim + 4 * lane);
+    __shared__ float factor[kMaxSplits];
+    __shared__ float wave_top[4], wave_sum[4];
+    __shared__ f32x4 group_acc[8][32];
+    const int64_t at = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = threadIdx.x;
+    float top = kNoMax, sum = 0.f;
+    if (p < parts.splits) {
+        top = parts.stat[2 * (p * parts.rows + at)];
+        sum = parts.stat[2 * (p * parts.rows + at) + 1];
+    }
+    float all = top;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = fmaf(x[e], f, acc[e]);
+    for (int d = 32; d > 0; d >>= 1) all = fmaxf(all, __shfl_xor(all, d));
+    if (lane == 0) wave_top[wave] = all;
+    __syncthreads();
+    all = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+    const float f = exp2_(top - all);
+    if (p < parts.splits) factor[p] = f;
+    sum *= f;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) wave_sum[wave] = sum;
+    __syncthreads();
+    sum = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+
+    const int group = threadIdx.x >> 5, c = 4 * (threadIdx.x & 31);
+    f32x4 acc = {};
+    if (c < a.dim) {
+#pragma unroll 4
+        for (int s = group; s < parts.splits; s += 8) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(parts.out + (s * parts.rows + at) * a.dim + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(x[e], factor[s], acc[e]);
         }
     }
+    group_acc[group][threadIdx.x & 31] = acc;
+    __syncthreads();
+    if (group > 0) return;
     const int i = static_cast<int>(at % a.nq);
     const int64_t bh = at / a.nq;
     const int head = static_cast<int>(bh % a.heads);
     const int64_t b = bh / a.heads;
-    if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-    if (4 * lane >= a.dim) return;
+    if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2;
+    if (c >= a.dim) return;
+#pragma unroll
+    for (int g = 1; g < 8; ++g) acc += group_acc[g][threadIdx.x];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[e] * inv);
-    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head + 4 * lane) = o;
+    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head + c) = o;
 }
 
 template <typename T>
@@ -285,7 +312,7 @@ void launch(const ddpm_span_attention_args& a, const Plan& plan, void* workspace
         else
             fwd_kernel<T, decltype(dp)::value, false><<<grid, kThreads, 0, stream>>>(d, plan.pack, parts);
     });
-    if (plan.splits > 1) join_kernel<T><<<static_cast<unsigned>((parts.rows + 3) / 4), 256, 0, stream>>>(d, parts);
+    if (plan.splits > 1) join_kernel<T><<<static_cast<unsigned>(parts.rows), 256, 0, stream>>>(d, parts);
 }
 
 }  // namespace

@@ -19,8 +19,8 @@ from ._lib import call, lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # DDPM_F32, DDPM_BF16, DDPM_F16
 _NORMS = {2.0: 0, math.inf: 1}                                        # DDPM_NORM_2, DDPM_NORM_MAX
-_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-_dtype, _device = attrgetter("dtype"), attrgetter("device")
+_ptr, _numel, _contiguous, _gpu = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype, _grad = attrgetter("dtype"), attrgetter("grad")
 
 
 def _array(code, values):
@@ -34,37 +34,44 @@ def _stream(device):
 
 
 def _one_gpu(what, tensors):
-    devices = set(map(_device, tensors))
-    if len(devices) != 1 or next(iter(devices)).type != "cuda":
-        raise RuntimeError(f"{what} (HIP): all tensors must be on one GPU, got {sorted(map(str, devices))}")
-    return next(iter(devices))
+    """Index of the GPU that all of them are on."""
+    gpus = set(map(_gpu, tensors))
+    if len(gpus) != 1 or -1 in gpus:
+        raise RuntimeError(f"{what} (HIP): all tensors must be on one GPU, got {sorted(str(t.device) for t in tensors)[:4]}")
+    return gpus.pop()
+
+
+def _distinct(what, pointers, sizes):
+    """Tensors that a kernel writes must not be given twice; empty ones may share a pointer."""
+    if len(set(pointers)) < len(pointers):
+        real = [p for p, n in zip(pointers, sizes) if n]
+        if len(set(real)) < len(real):
+            raise ValueError(f"{what} (HIP): the same tensor is given twice")
 
 
 class _Norm:
     """The gradients of one call as the C arrays of the norm and clipping entry points, and the norm itself:
-    `state` holds [norm, factor] on the device."""
+    `state` holds [norm, factor] on the device. They must be contiguous; where the caller has their pointers and sizes already
+    it hands them in."""
 
-    def __init__(self, what, grads, max_norm, norm_type):
+    def __init__(self, what, grads, max_norm, norm_type, pointers=None, sizes=None):
         if norm_type not in _NORMS:
             raise NotImplementedError(f"{what} (HIP): norm_type must be 2 or inf, got {norm_type}")
         if not max_norm >= 0.0:
             raise ValueError(f"Invalid max_norm: {max_norm}")
         self.device = _one_gpu(what, grads)
-        if not all(map(_contiguous, grads)):
-            raise RuntimeError(f"{what} (HIP): gradients must be contiguous")
         types = list(map(_TYPES.get, map(_dtype, grads)))
         if None in types:
             raise RuntimeError(f"{what} (HIP): gradients must be float32, bfloat16 or float16, got {sorted(map(str, set(map(_dtype, grads))))}")
         self.n = len(grads)
-        numel = list(map(_numel, grads))
-        pointers = list(map(_ptr, grads))
-        if len(set(pointers)) < self.n and len({p for p, k in zip(pointers, numel) if k}) < sum(map(bool, numel)):
-            raise ValueError(f"{what} (HIP): the same gradient is given twice")
-        (self.pointers, a), (self.numel, b), (self.types, c) = _array("Q", pointers), _array("q", numel), _array("i", types)
+        if pointers is None:
+            pointers, sizes = list(map(_ptr, grads)), list(map(_numel, grads))
+            _distinct(what, pointers, sizes)
+        (self.pointers, a), (self.numel, b), (self.types, c) = _array("Q", pointers), _array("q", sizes), _array("i", types)
         self._owners = (a, b, c)
         with torch.cuda.device(self.device):
-            workspace = torch.empty(lib().ddpm_grad_norm_workspace_doubles(self.n), dtype=torch.float64, device=self.device)
-            self.state = torch.empty(2, dtype=torch.float32, device=self.device)
+            workspace = torch.empty(lib().ddpm_grad_norm_workspace_doubles(self.n), dtype=torch.float64, device="cuda")
+            self.state = torch.empty(2, dtype=torch.float32, device="cuda")
             call("ddpm_grad_norm", self.n, self.pointers, self.numel, self.types, _NORMS[norm_type], float(max_norm),
                  C.c_void_p(workspace.data_ptr()), C.c_void_p(self.state.data_ptr()), _stream(self.device))
 
@@ -73,19 +80,20 @@ class _Norm:
 
 
 def _gradients(what, parameters):
+    """(gradients, the same contiguous)"""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
-    if any(g.is_sparse for g in grads):
+    grads = [g for g in map(_grad, parameters) if g is not None]
+    if any(g.layout != torch.strided for g in grads):
         raise RuntimeError(f"{what} does not support sparse gradients")
-    return grads
+    return grads, grads if all(map(_contiguous, grads)) else [g.contiguous() for g in grads]
 
 
 @torch.no_grad()
 def grad_norm(parameters, norm_type=2.0):
     """Norm of all gradients of `parameters` together (a 0-dim fp32 tensor on their GPU): the 2-norm, summed in float64
     in a fixed order, or with norm_type=inf the largest magnitude. The gradients stay as they are."""
-    grads = [g if g.is_contiguous() else g.contiguous() for g in _gradients("grad_norm", parameters)]
+    _, grads = _gradients("grad_norm", parameters)
     return _Norm("grad_norm", grads, math.inf, float(norm_type)).state[0] if grads else torch.tensor(0.0)
 
 
@@ -94,31 +102,32 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """torch.nn.utils.clip_grad_norm_ over fp32, bf16 and fp16 gradients on one GPU: scales all of them in place by
     min(1, max_norm / (norm + 1e-6)) and returns the norm before (0-dim fp32, on the device; nothing waits for it unless
     error_if_nonfinite is set). A norm that is not a number makes every gradient NaN, as there."""
-    grads = _gradients("clip_grad_norm_", parameters)
+    grads, dense = _gradients("clip_grad_norm_", parameters)
     if not grads:
         return torch.tensor(0.0)
-    dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
     norm = _Norm("clip_grad_norm_", dense, max_norm, float(norm_type))
     if error_if_nonfinite and not math.isfinite(norm.state[0].item()):
         raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
     with torch.cuda.device(norm.device):
         call("ddpm_clip_grads", norm.n, norm.pointers, norm.numel, norm.types, norm.factor(), _stream(norm.device))
-        for g, d in zip(grads, dense):
-            if g is not d:
-                g.copy_(d)
+        if dense is not grads:
+            for g, d in zip(grads, dense):
+                if g is not d:
+                    g.copy_(d)
     torch.autograd.graph.increment_version(grads)
     return norm.state[0]
 
 
-def _update(lists, step, lr, beta1, beta2, eps, weight_decay, factor):
+def _update(lists, pointers, sizes, step, lr, beta1, beta2, eps, weight_decay, factor):
     """Launches the update of checked lists (parameters, gradients, exp_avg, exp_avg_sq) on the current GPU and stream."""
-    arrays = [_array("Q", map(_ptr, x)) for x in lists]
-    numel = _array("q", map(_numel, lists[0]))
-    args = (len(lists[0]), *(a[0] for a in arrays), numel[0], float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), step)
+    arrays = [_array("Q", x) for x in pointers]
+    numel = _array("q", sizes)
+    args = (len(sizes), *(a[0] for a in arrays), numel[0], float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), step)
+    stream = _stream(torch.cuda.current_device())
     if factor is None:
-        call("ddpm_adam_step", *args, _stream(lists[0][0].device))
+        call("ddpm_adam_step", *args, stream)
     else:
-        call("ddpm_adam_step_clipped", *args, factor, _stream(lists[0][0].device))
+        call("ddpm_adam_step_clipped", *args, factor, stream)
     # the kernel wrote the tensors behind autograd's back: record the in-place change, as any in-place
     # torch op would (saved-tensor checks and caches keyed on the version counter rely on it)
     torch.autograd.graph.increment_version(list(chain(lists[0], lists[2], lists[3])))
@@ -129,25 +138,25 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     """One Adam update of lists of contiguous fp32 tensors on one GPU, in place; `step` counts from 1, this update
     included. With max_norm the gradients count as if clip_grad_norm_(max_norm) had scaled them first; they themselves stay
     as they are, and their norm is returned (0-dim fp32 on the device; None without max_norm)."""
-    params, grads, exp_avgs, exp_avg_sqs = lists = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs)]
+    lists = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs)]
     if len(set(map(len, lists))) != 1:
         raise ValueError(f"adam_step_: lists of different lengths {[len(x) for x in lists]}")
     if step < 1:
         raise ValueError(f"Invalid step: {step}")
-    if not params:
+    if not lists[0]:
         return None
     every = list(chain(*lists))
-    device = _one_gpu("adam_step_", every)
+    gpu = _one_gpu("adam_step_", every)
     if set(map(_dtype, every)) != {torch.float32} or not all(map(_contiguous, every)):
         raise RuntimeError("adam_step_ (HIP): all tensors must be contiguous fp32")
-    if any(len(set(x)) != 1 for x in zip(*(map(_numel, x) for x in lists))):
+    sizes = list(map(_numel, lists[0]))
+    if any(list(map(_numel, x)) != sizes for x in lists[1:]):
         raise RuntimeError("adam_step_ (HIP): gradients and moments must match their parameters in size")
-    written = [t.data_ptr() for t in chain(params, exp_avgs, exp_avg_sqs) if t.numel()]
-    if len(set(written)) < len(written):
-        raise ValueError("adam_step_ (HIP): the same tensor is given twice")
-    norm = _Norm("adam_step_", grads, max_norm, 2.0) if max_norm is not None else None
-    with torch.cuda.device(device):
-        _update(lists, int(step), lr, *betas, eps, weight_decay, norm and norm.factor())
+    pointers = [list(map(_ptr, x)) for x in lists]
+    _distinct("adam_step_", pointers[0] + pointers[2] + pointers[3], sizes * 3)
+    with torch.cuda.device(gpu):
+        norm = _Norm("adam_step_", lists[1], max_norm, 2.0, pointers[1], sizes) if max_norm is not None else None
+        _update(lists, pointers, sizes, int(step), lr, *betas, eps, weight_decay, norm and norm.factor())
     return norm and norm.state[0]
 
 
@@ -207,7 +216,8 @@ class Adam(torch.optim.Optimizer):
             self.grad_norm = norm.state[0]
         for group, step, items in work:
             with torch.cuda.device(items[0][0].device):
-                _update([list(x) for x in zip(*items)], step, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
+                lists = [list(x) for x in zip(*items)]
+                _update(lists, [list(map(_ptr, x)) for x in lists], list(map(_numel, lists[0])), step, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
                         norm and norm.factor())
             for p, *_ in items:
                 self.state[p]["step"] += 1
