@@ -90,6 +90,18 @@ __device__ __forceinline__ float other_half(float x) {
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------------
+// Rows of DP channels without gaps (loads from memory to LDS write 1 KiB of neighbouring lanes), their 16-byte chunks exchanged
+// by row: chunk c of a row lies at c ^ swizzle(row). In units of 64 bytes the four rows of a transposing read then fall into the
+// four different quarters of the 256 bytes of banks, and 16 rows read at one chunk (dot) into 16 different chunks of them.
+// With 8 channels of padding instead, both kinds of reads met conflicts.
+template <typename T, int DP>
+__device__ __forceinline__ constexpr int swizzle(int row) {
+    constexpr int chunks = DP * static_cast<int>(sizeof(T)) / 16;
+    if (sizeof(T) == 4) return row & 7;
+    return ((row >> 2) & 3) | (chunks == 16 ? (row & 3) << 2 : chunks == 8 ? ((row >> 1) & 1) << 2 : 0);
+}
+
 // ---- matrix products of a type ---------------------------------------------------------------------------------------
 template <typename T>
 struct Ops {                             // bf16, fp16
@@ -117,20 +129,22 @@ struct Ops {                             // bf16, fp16
         return w;
     }
     // acc[db] += over 32 tile rows; `tile` points at the first of them
-    template <int DP, int PITCH>
+    template <int DP>
     static __device__ __forceinline__ void spread(f32x16* acc, const T* tile, const Weights& w) {
         // The transposing read gives lane l of 16 the column l of a 4 x 16 block whose rows four lanes each point at: rows
         // 4 h ... 4 h + 3 (and 8 further) are the ones whose weights this lane half holds.
-        const int lane = threadIdx.x & 63, l16 = lane & 15;
-        const T* at = tile + (4 * (lane >> 5) + (l16 >> 2)) * PITCH + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
+        const int lane = threadIdx.x & 63, l16 = lane & 15, row = 4 * (lane >> 5) + (l16 >> 2);
+        const int chunk = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
+        const T* at = tile + row * DP + 4 * (l16 & 1);
+        const int swap0 = swizzle<T, DP>(row), swap1 = swizzle<T, DP>(row + 8);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) {
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4*)(at + 16 * t * PITCH + 32 * db));
+                    (__attribute__((address_space(3))) s16x4*)(at + 16 * t * DP + W * ((4 * db + chunk) ^ swap0)));
                 const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4*)(at + (16 * t + 8) * PITCH + 32 * db));
+                    (__attribute__((address_space(3))) s16x4*)(at + (16 * t + 8) * DP + W * ((4 * db + chunk) ^ swap1)));
                 const auto xy = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[db] = mfma(__builtin_bit_cast(Frag, xy), w.f[t], acc[db]);
             }
@@ -153,23 +167,19 @@ struct Ops<float> {
         return c;
     }
     static __device__ __forceinline__ Weights pack(const f32x16& p) { return p; }
-    template <int DP, int PITCH>
+    template <int DP>
     static __device__ __forceinline__ void spread(f32x16* acc, const float* tile, const Weights& w) {
-        const int lane = threadIdx.x & 63;
-        const float* at = tile + 4 * (lane >> 5) * PITCH + (lane & 31);
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        const float* at = tile + 4 * half * DP + (lane & 3);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
+        for (int r = 0; r < 16; ++r) {
+            const int row = 8 * (r >> 2) + (r & 3), swap = swizzle<float, DP>(4 * half + row);
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * PITCH + 32 * db], w[r], acc[db], 0, 0, 0);
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[row * DP + 32 * db + 4 * (((lane >> 2) & 7) ^ swap)], w[r], acc[db], 0, 0, 0);
+        }
     }
 };
-
-// row pitch of a tile in LDS: 16 bytes beyond the row, so that the 32 rows a dot reads at once start in different banks
-template <typename T, int DP>
-constexpr int pitch() {
-    return DP + Ops<T>::W;
-}
 
 // the lane's own row: channels kStep s + W h ... of step s, nought behind dim
 template <typename T, int DP>
@@ -187,41 +197,39 @@ struct OwnRow {
         }
     }
     // product with 32 tile rows
-    template <int PITCH>
     __device__ __forceinline__ f32x16 dot(const T* tile) const {
-        const int lane = threadIdx.x & 63;
-        const T* at = tile + (lane & 31) * PITCH + Ops<T>::W * (lane >> 5);
+        const int lane = threadIdx.x & 63, row = lane & 31, swap = swizzle<T, DP>(row) ^ (lane >> 5);
         f32x16 acc = {};
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) acc = Ops<T>::mul(*reinterpret_cast<const typename Ops<T>::Frag*>(at + Ops<T>::kStep * s), f[s], acc);
+        for (int s = 0; s < kSteps; ++s)
+            acc = Ops<T>::mul(*reinterpret_cast<const typename Ops<T>::Frag*>(tile + row * DP + Ops<T>::W * ((2 * s) ^ swap)), f[s], acc);
         return acc;
     }
 };
 
-// kTile rows on their way from memory to LDS. Rows outside [lo, hi) read the nearest row inside: they are masked, and what
-// memory holds behind a sequence is not looked at. Channels behind dim become noughts.
+// Starts the loads of kTile rows from memory to LDS; they have arrived behind the next arrived(). Rows outside [lo, hi) read
+// the nearest row inside: they are masked, and what memory holds behind a sequence is not looked at. Chunks behind dim
+// read the row's first one: their products with the noughts of an OwnRow are nought, and channels there are not written.
 template <typename T, int DP>
-struct Staged {
-    static constexpr int kChunks = DP / Ops<T>::W, kLoads = Ops<T>::kTile * kChunks / kThreads;
-    typename Ops<T>::Frag r[kLoads];
+__device__ __forceinline__ void fetch(T* tile, const T* base, int64_t row_stride, int row0, int lo, int hi, int dim) {
+    constexpr int W = Ops<T>::W, kChunks = DP / W, kLoads = Ops<T>::kTile * kChunks / kThreads;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int first = (wave * kLoads + i) * 64, id = first + (threadIdx.x & 63), row = id / kChunks;
+        const int c = W * ((id - row * kChunks) ^ swizzle<T, DP>(row));
+        const int at = min(max(row0 + row, lo), hi - 1);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(base + at * row_stride + (c < dim ? c : 0)),
+                                         (__attribute__((address_space(3))) unsigned*)(tile + first * W), 16, 0, 0);
+    }
+}
 
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int row0, int lo, int hi, int dim) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, c = (idx - row * kChunks) * Ops<T>::W;
-            const int at = min(max(row0 + row, lo), hi - 1);
-            r[i] = *reinterpret_cast<const typename Ops<T>::Frag*>(base + at * row_stride + (c < dim ? c : 0));
-        }
-    }
-    __device__ __forceinline__ void store(T* tile, int dim) const {
-        constexpr int kPitch = pitch<T, DP>();
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, c = (idx - row * kChunks) * Ops<T>::W;
-            *reinterpret_cast<typename Ops<T>::Frag*>(tile + row * kPitch + c) = c < dim ? r[i] : typename Ops<T>::Frag{};
-        }
-    }
-};
+// Barrier behind which every wave's fetches are in LDS. __syncthreads() alone does not wait for them: they count as loads from
+// memory, which a workgroup's fence leaves in flight.
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
 
 // ---- scores ------------------------------------------------------------------------------------------------------------
 // From q.k to log2(e) u: with a cap, cap log2(e) tanh(scale q.k / cap).

@@ -59,10 +59,9 @@ __device__ __forceinline__ void write_row(T* out, const f32x16* acc, float f, in
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_kernel(const Dev a, const Work work) {
-    constexpr int kPitch = pitch<T, DP>(), kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+    constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
     constexpr bool kGain = __is_same(T, _Float16);
-    __shared__ __attribute__((aligned(16))) T k_tile[kTile * kPitch];
-    __shared__ __attribute__((aligned(16))) T v_tile[kTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) T k_even[kTile * DP], k_odd[kTile * DP], v_even[kTile * DP], v_odd[kTile * DP];
     __shared__ int bounds[2][4];
 
     const dim3 id = ddpm::xcd_block();
@@ -116,27 +115,23 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     const T* v = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
     f32x16 acc[DP / 32] = {};
     float gain = gain_for(0.f), largest = 0.f;
-    Staged<T, DP> ks, vs;
     if (first < last) {
-        ks.load(k, a.sk.row, first * kTile, lo, hi, a.dim);
-        vs.load(v, a.sv.row, first * kTile, lo, hi, a.dim);
+        fetch<T, DP>(k_even, k, a.sk.row, first * kTile, lo, hi, a.dim);
+        fetch<T, DP>(v_even, v, a.sv.row, first * kTile, lo, hi, a.dim);
     }
-    for (int t = first; t < last; ++t) {
-        __syncthreads();
-        ks.store(k_tile, a.dim);
-        vs.store(v_tile, a.dim);
-        __syncthreads();
+    const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
+        arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
         if (t + 1 < last) {
-            ks.load(k, a.sk.row, j0 + kTile, lo, hi, a.dim);
-            vs.load(v, a.sv.row, j0 + kTile, lo, hi, a.dim);
+            fetch<T, DP>(k_next, k, a.sk.row, j0 + kTile, lo, hi, a.dim);
+            fetch<T, DP>(v_next, v, a.sv.row, j0 + kTile, lo, hi, a.dim);
         }
-        if (j0 + kTile <= wlo || j0 >= whi) continue;
+        if (j0 + kTile <= wlo || j0 >= whi) return;
         const bool whole = __all(row.lo <= j0 && row.hi >= j0 + kTile);
 #pragma unroll
         for (int kb = 0; kb < kBlocks; ++kb) {
-            f32x16 s = q.template dot<kPitch>(k_tile + kb * 32 * kPitch);
-            const f32x16 dp = dout.template dot<kPitch>(v_tile + kb * 32 * kPitch);
+            f32x16 s = q.dot(k_now + kb * 32 * DP);
+            const f32x16 dp = dout.dot(v_now + kb * 32 * DP);
             score.apply<T>(s);
             f32x16 ds;
 #pragma unroll
@@ -163,8 +158,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
                 }
                 ds *= gain;
             }
-            Ops<T>::template spread<DP, kPitch>(acc, k_tile + kb * 32 * kPitch, Ops<T>::pack(ds));
+            Ops<T>::template spread<DP>(acc, k_now + kb * 32 * DP, Ops<T>::pack(ds));
         }
+    };
+    for (int t = first; t < last; t += 2) {          // both buffers written out, as in the forward kernel
+        step(t, k_even, v_even, k_odd, v_odd);
+        if (t + 1 < last) step(t + 1, k_odd, v_odd, k_even, v_even);
     }
     if constexpr (kGain) {
 #pragma unroll
@@ -175,27 +174,36 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
         write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, kGain ? inverse_gain(gain) : 1.f, a.dim);
 }
 
-// The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other.
+// The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other. A lane holds what one of 64
+// tiles sees, so that going on needs no memory (a load behind the fetches of a tile could only arrive after them).
 template <int GROUPS>                    // groups of 32 rows in a tile
 struct Tiles {
     const Seen* seen;
     int groups, tiles, heads, begin, end;
-    int head, base;                      // 64 tiles from `base` on are in `mask`
+    int base;                            // 64 tiles from `base` on are in `mask` and `mine`
     unsigned long long mask;
+    Seen mine[GROUPS];
+    // the current one
+    int head, tile;
+    Seen now[GROUPS];
 
     __device__ __forceinline__ void look() {
         const int t = base + (threadIdx.x & 63);
         bool any = false;
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-            if (t * GROUPS + g < groups) {
-                const Seen s = seen[t * GROUPS + g];
-                any |= s.lo < end && s.hi > begin;
-            }
+        for (int g = 0; g < GROUPS; ++g) {
+            mine[g] = {INT32_MAX, 0, INT32_MAX, 0};
+            if (t * GROUPS + g < groups) mine[g] = seen[t * GROUPS + g];
+            any |= mine[g].lo < end && mine[g].hi > begin;
+        }
         mask = __ballot(any);
     }
+    __device__ __forceinline__ void start() {
+        base = head = 0;
+        look();
+    }
     // moves to the next tile; false behind the last one
-    __device__ __forceinline__ bool next(int& h, int& tile) {
+    __device__ __forceinline__ bool next() {
         while (mask == 0) {
             base += 64;
             if (base >= tiles) {
@@ -204,22 +212,28 @@ struct Tiles {
             }
             look();
         }
-        tile = base + __builtin_ctzll(mask);
+        const int lane = __builtin_ctzll(mask);
         mask &= mask - 1;
-        h = head;
+        tile = base + lane;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            now[g].lo = __builtin_amdgcn_readlane(mine[g].lo, lane);
+            now[g].hi = __builtin_amdgcn_readlane(mine[g].hi, lane);
+            now[g].all_lo = __builtin_amdgcn_readlane(mine[g].all_lo, lane);
+            now[g].all_hi = __builtin_amdgcn_readlane(mine[g].all_hi, lane);
+        }
         return true;
     }
 };
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const Dev a, const Work work) {
-    constexpr int kPitch = pitch<T, DP>(), kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+    constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
     constexpr bool kGain = __is_same(T, _Float16);
     constexpr float kUnshift = 1.f / (1 << Ops<T>::kShift);
-    __shared__ __attribute__((aligned(16))) T q_tile[kTile * kPitch];
-    __shared__ __attribute__((aligned(16))) T do_tile[kTile * kPitch];
-    __shared__ __attribute__((aligned(16))) float stat_tile[kTile], delta_tile[kTile];
-    __shared__ __attribute__((aligned(16))) int lo_tile[kTile], hi_tile[kTile], pos_tile[kTile];
+    __shared__ __attribute__((aligned(1024))) T q_even[kTile * DP], q_odd[kTile * DP], do_even[kTile * DP], do_odd[kTile * DP];
+    __shared__ __attribute__((aligned(16))) float stat_tile[2][kTile], delta_tile[2][kTile];
+    __shared__ __attribute__((aligned(16))) int lo_tile[2][kTile], hi_tile[2][kTile], pos_tile[2][kTile];
     __shared__ float wave_max[4];
 
     const dim3 id = ddpm::xcd_block();
@@ -252,29 +266,15 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
     tiles.heads = a.group;
     tiles.begin = begin;
     tiles.end = min(begin + kRows, a.nk);
-    tiles.head = tiles.base = 0;
-    tiles.look();
+    tiles.start();
 
-    Staged<T, DP> qs, dos;
+    // Of the tile that `tiles` stands at: what its rows see, their lse and their D, into registers and then (write_rows) into LDS, and
+    // the loads of its q and dout, in this order, so that the registers do not have to wait for the tile.
     Row row = no_row();
-    float stat = 0.f, delta = 0.f;
-    bool dead[Staged<T, DP>::kLoads];    // rows that see nothing: what q and dout hold there is not looked at
-    const auto load = [&](int h, int tile) {
-        const int head = kv * a.group + h, i0 = tile * kTile;
-        qs.load(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, a.sq.row, i0, 0, a.nq, a.dim);
-        dos.load(static_cast<const T*>(a.dout) + b * a.sdo.batch + head * a.sdo.head, a.sdo.row, i0, 0, a.nq, a.dim);
-        bool all = true;
-#pragma unroll
-        for (int g = 0; g < kBlocks; ++g)
-            if (tile * kBlocks + g < work.groups) all &= tiles.seen[tile * kBlocks + g].all_lo != INT32_MAX;
-#pragma unroll
-        for (int x = 0; x < Staged<T, DP>::kLoads; ++x) {
-            dead[x] = false;
-            if (!all) {
-                const int i = i0 + (x * kThreads + static_cast<int>(threadIdx.x)) / Staged<T, DP>::kChunks;
-                dead[x] = i >= a.nq || row_of(a, b, i).hi == 0;
-            }
-        }
+    float stat = 0.f, delta = 0.f, next_slope = 0.f;
+    const auto load = [&](T* q_to, T* do_to) __attribute__((always_inline)) {
+        const int head = kv * a.group + tiles.head, i0 = tiles.tile * kTile;
+        if (a.slopes) next_slope = a.slopes[head] * kLog2e;
         if (threadIdx.x < kTile) {
             const int i = i0 + threadIdx.x;
             row = no_row();
@@ -283,63 +283,79 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
             if (i < a.nq) {
                 const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
                 row = row_of(a, b, i);
-                stat = stat_of(a.lse[at]);
+                stat = a.lse[at];
                 delta = work.delta[at];
             }
         }
+        fetch<T, DP>(q_to, static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, a.sq.row, i0, 0, a.nq, a.dim);
+        fetch<T, DP>(do_to, static_cast<const T*>(a.dout) + b * a.sdo.batch + head * a.sdo.head, a.sdo.row, i0, 0, a.nq, a.dim);
+    };
+    const auto write_rows = [&](int to) __attribute__((always_inline)) {
+        if (threadIdx.x < kTile) {
+            lo_tile[to][threadIdx.x] = row.lo;
+            hi_tile[to][threadIdx.x] = row.hi;
+            pos_tile[to][threadIdx.x] = row.pos;
+            stat_tile[to][threadIdx.x] = stat_of(stat);
+            delta_tile[to][threadIdx.x] = delta;
+        }
     };
 
-    int h = 0, tile = 0;
-    bool more = tiles.next(h, tile);
-    if (more) load(h, tile);
-    while (more) {
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < Staged<T, DP>::kLoads; ++x)
-            if (dead[x]) qs.r[x] = dos.r[x] = typename Ops<T>::Frag{};
-        qs.store(q_tile, a.dim);
-        dos.store(do_tile, a.dim);
-        if (threadIdx.x < kTile) {
-            lo_tile[threadIdx.x] = row.lo;
-            hi_tile[threadIdx.x] = row.hi;
-            pos_tile[threadIdx.x] = row.pos;
-            stat_tile[threadIdx.x] = stat;
-            delta_tile[threadIdx.x] = delta;
-        }
-        __syncthreads();
-        const int now = tile, head = kv * a.group + h;
-        more = tiles.next(h, tile);
-        if (more) load(h, tile);
-        const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    bool more = tiles.next();
+    if (more) {
+        load(q_even, do_even);
+        write_rows(0);
+    }
+    const auto step = [&](int in, T* q_now, T* do_now, T* q_next, T* do_next) __attribute__((always_inline)) {
+        arrived();                       // this tile is here, the one before is done with
+        const float slope = next_slope;
+        Seen now[kBlocks];
+        bool all = true;                 // does every row see some key?
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g) {
-            if (now * kBlocks + g >= work.groups) continue;
-            const Seen seen = tiles.seen[now * kBlocks + g];
-            if (seen.lo >= w0 + 32 || seen.hi <= w0) continue;
-            const bool whole = seen.all_lo <= w0 && seen.all_hi >= w0 + 32;
-            f32x16 s = k.template dot<kPitch>(q_tile + g * 32 * kPitch);
-            const f32x16 dp = v.template dot<kPitch>(do_tile + g * 32 * kPitch);
+            now[g] = tiles.now[g];
+            all &= now[g].all_lo != INT32_MAX;
+        }
+        more = tiles.next();
+        if (more) load(q_next, do_next);
+        if (!all) {                      // what q and dout hold in a row that sees none does not matter: noughts
+            constexpr int kChunks = DP / Ops<T>::W;
+            for (int x = threadIdx.x; x < kTile * kChunks; x += kThreads)
+                if (hi_tile[in][x / kChunks] == 0)
+                    reinterpret_cast<typename Ops<T>::Frag*>(q_now)[x] = reinterpret_cast<typename Ops<T>::Frag*>(do_now)[x] = {};
+            __syncthreads();
+        }
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g) {
+            if (now[g].lo >= w0 + 32 || now[g].hi <= w0) continue;
+            const bool whole = now[g].all_lo <= w0 && now[g].all_hi >= w0 + 32;
+            f32x16 s = k.dot(q_now + g * 32 * DP);
+            const f32x16 dp = v.dot(do_now + g * 32 * DP);
             score.apply<T>(s);
             f32x16 p, ds;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int at = 32 * g + 8 * x + 4 * half;              // four rows
-                const f32x4 stats = *reinterpret_cast<const f32x4*>(stat_tile + at);
-                const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile + at);
+                const f32x4 stats = *reinterpret_cast<const f32x4*>(stat_tile[in] + at);
+                const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile[in] + at);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float w = s[4 * x + e] + Ops<T>::kShift - stats[e];
-                    if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(pos_tile[at + e] - j)), w);
+                    if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(pos_tile[in][at + e] - j)), w);
                     float y = exp2_(w), d = y * (dp[4 * x + e] - deltas[e]) * (a.scale * kUnshift);
                     if (score.capped) d *= score.slope(s[4 * x + e]);
-                    if (!whole && (j < lo_tile[at + e] || j >= hi_tile[at + e])) y = d = 0.f;
+                    if (!whole && (j < lo_tile[in][at + e] || j >= hi_tile[in][at + e])) y = d = 0.f;
                     p[4 * x + e] = y;
                     ds[4 * x + e] = kGain ? d * gain : d;
                 }
             }
-            Ops<T>::template spread<DP, kPitch>(dv, do_tile + g * 32 * kPitch, Ops<T>::pack(p));
-            Ops<T>::template spread<DP, kPitch>(dk, q_tile + g * 32 * kPitch, Ops<T>::pack(ds));
+            Ops<T>::template spread<DP>(dv, do_now + g * 32 * DP, Ops<T>::pack(p));
+            Ops<T>::template spread<DP>(dk, q_now + g * 32 * DP, Ops<T>::pack(ds));
         }
+        if (more) write_rows(in ^ 1);
+    };
+    while (more) {                       // both buffers written out, as in the forward kernel
+        step(0, q_even, do_even, q_odd, do_odd);
+        if (more) step(1, q_odd, do_odd, q_even, do_even);
     }
     if (!real) return;
     write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, kGain ? inverse_gain(gain) : 1.f, a.dim);

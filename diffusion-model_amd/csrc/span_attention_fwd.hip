@@ -1,7 +1,7 @@
 // Span attention, forward (the mathematics and the two products are in span_attention.h).
 //
 // A workgroup of 4 waves takes 128 rows of one head, 32 a wave, and walks over the keys that any of them sees, a tile of 64
-// (fp32: 32) at a time: k and v go through registers into LDS, the next tile's loads fly while this one is worked on, and a
+// (fp32: 32) at a time: k and v go straight into LDS, the next tile's while this one is worked on, and a
 // running maximum and sum turn the scores into weights in one pass. With few rows (single tokens) the query heads that share
 // a key/value head are rows of one workgroup, and the keys are split over workgroups whose parts a second kernel joins.
 #include <algorithm>
@@ -96,9 +96,8 @@ struct Parts {                           // of a split call: per part and row th
 
 template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int pack, const Parts parts) {
-    constexpr int kPitch = pitch<T, DP>(), kTile = Ops<T>::kTile, kBlocks = kTile / 32;
-    __shared__ __attribute__((aligned(16))) T k_tile[kTile * kPitch];
-    __shared__ __attribute__((aligned(16))) T v_tile[kTile * kPitch];
+    constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+    __shared__ __attribute__((aligned(1024))) T k_even[kTile * DP], k_odd[kTile * DP], v_even[kTile * DP], v_odd[kTile * DP];
     __shared__ int bounds[2][4];
 
     // x: row blocks (the last first: under causal order they have most to do), and with SPLIT the parts of the keys beside them
@@ -140,26 +139,22 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
 
     f32x16 acc[DP / 32] = {};
     float top = kNoMax, sum = 0.f;       // of this column: maximum of all its scores, sum of this lane half's weights
-    Staged<T, DP> ks, vs;
     if (first < last) {
-        ks.load(k, a.sk.row, first * kTile, lo, hi, a.dim);
-        vs.load(v, a.sv.row, first * kTile, lo, hi, a.dim);
+        fetch<T, DP>(k_even, k, a.sk.row, first * kTile, lo, hi, a.dim);
+        fetch<T, DP>(v_even, v, a.sv.row, first * kTile, lo, hi, a.dim);
     }
-    for (int t = first; t < last; ++t) {
-        __syncthreads();
-        ks.store(k_tile, a.dim);
-        vs.store(v_tile, a.dim);
-        __syncthreads();
+    const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
+        arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
         if (t + 1 < last) {
-            ks.load(k, a.sk.row, j0 + kTile, lo, hi, a.dim);
-            vs.load(v, a.sv.row, j0 + kTile, lo, hi, a.dim);
+            fetch<T, DP>(k_next, k, a.sk.row, j0 + kTile, lo, hi, a.dim);
+            fetch<T, DP>(v_next, v, a.sv.row, j0 + kTile, lo, hi, a.dim);
         }
-        if (j0 + kTile <= wlo || j0 >= whi) continue;               // nothing here for this wave's rows
+        if (j0 + kTile <= wlo || j0 >= whi) return;                 // nothing here for this wave's rows
         f32x16 s[kBlocks];
 #pragma unroll
         for (int kb = 0; kb < kBlocks; ++kb) {
-            s[kb] = q.template dot<kPitch>(k_tile + kb * 32 * kPitch);
+            s[kb] = q.dot(k_now + kb * 32 * DP);
             score.apply<T>(s[kb]);
         }
         if (a.slopes) {
@@ -200,8 +195,14 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
                 s[kb][e] = exp2_(s[kb][e] + shift);
                 sum += s[kb][e];
             }
-            Ops<T>::template spread<DP, kPitch>(acc, v_tile + kb * 32 * kPitch, Ops<T>::pack(s[kb]));
+            Ops<T>::template spread<DP>(acc, v_now + kb * 32 * DP, Ops<T>::pack(s[kb]));
         }
+    };
+    // The two buffers are variables of their own, and the loop is written out for both: with one indexed by t the compiler has to
+    // assume that a read of this tile may meet the loads of the next, and waits for them at once.
+    for (int t = first; t < last; t += 2) {
+        step(t, k_even, v_even, k_odd, v_odd);
+        if (t + 1 < last) step(t + 1, k_odd, v_odd, k_even, v_even);
     }
 
     sum += other_half(sum);
