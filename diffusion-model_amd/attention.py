@@ -62,8 +62,9 @@ def key_spans(rows, keys=None, *, documents=None, prefix=None, lengths=None, win
 
 
 def _fit(x, width):
-    """x, or a copy, with neighbouring channels on 16-byte boundaries."""
-    if x.stride(3) != 1 or x.data_ptr() % 16 or any(n > 1 and s % width for n, s in zip(x.shape[:3], x.stride())):
+    """x, or a copy, with neighbouring channels on 16-byte boundaries, and 64 rows within 2 GiB."""
+    if (x.stride(3) != 1 or x.data_ptr() % 16 or any(n > 1 and s % width for n, s in zip(x.shape[:3], x.stride()))
+            or x.shape[1] > 1 and x.stride(1) * x.element_size() >= 1 << 25):
         return x.clone(memory_format=torch.contiguous_format)
     return x
 

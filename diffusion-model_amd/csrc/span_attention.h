@@ -24,6 +24,7 @@ constexpr int kThreads = 256;            // 4 waves
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // running maximum before the first key: finite, so that its difference from -infinity (a masked score) is one
 constexpr float kNoMax = -1e30f;
+constexpr int kMaxTile = 64;             // rows of a tile, at most
 
 struct Strides {
     int64_t batch, row, head;
@@ -102,13 +103,29 @@ __device__ __forceinline__ constexpr int swizzle(int row) {
     return ((row >> 2) & 3) | (chunks == 16 ? (row & 3) << 2 : chunks == 8 ? ((row >> 1) & 1) << 2 : 0);
 }
 
+// Byte offset in a tile whose chunk is `delta` bytes (a constant) from that of `at`: an exclusive or as far as the exchange
+// reaches, which is the largest power of two in the row's length at most, and a sum above.
+template <typename T, int DP>
+__device__ __forceinline__ int chunk_from(int at, int delta) {
+    constexpr int bytes = DP * static_cast<int>(sizeof(T)), power = bytes & -bytes;
+    return (at ^ (delta & (power - 1))) + (delta & ~(power - 1));
+}
+
+template <typename V, typename T>
+__device__ __forceinline__ V read_at(const T* tile, int at) {
+    return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(tile) + at);
+}
+
 // ---- matrix products of a type ---------------------------------------------------------------------------------------
 template <typename T>
 struct Ops {                             // bf16, fp16
     typedef T Frag __attribute__((ext_vector_type(8)));
     static constexpr int W = 8;          // elements of 16 bytes
     static constexpr int kStep = 16;     // channels of one step of dot
-    static constexpr int kTile = 64;     // rows staged at a time
+    static constexpr int kTile = kMaxTile;   // rows in LDS at a time
+    // How far scores may pass the maximum that weights are relative to before sums are rescaled, in powers of two. Any number
+    // serves fp32's and bf16's exponents; fp16 has room for one beside kShift. With 0 some row of a wave has a new maximum in most tiles.
+    static constexpr float kSlack = __is_same(T, _Float16) ? 1.f : 8.f;
     // Weights are scaled by 2^kShift before they are rounded to T: fp16 has no more than 2^-24 at its small end, and a row of
     // thousands of keys has many weights below its normal numbers; bf16 has fp32's range.
     static constexpr int kShift = __is_same(T, _Float16) ? 14 : 0;
@@ -135,17 +152,16 @@ struct Ops {                             // bf16, fp16
         // 4 h ... 4 h + 3 (and 8 further) are the ones whose weights this lane half holds.
         const int lane = threadIdx.x & 63, l16 = lane & 15, row = 4 * (lane >> 5) + (l16 >> 2);
         const int chunk = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
-        const T* at = tile + row * DP + 4 * (l16 & 1);
-        const int swap0 = swizzle<T, DP>(row), swap1 = swizzle<T, DP>(row + 8);
+        const int at = 2 * row * DP + 16 * (chunk ^ swizzle<T, DP>(row)) + 8 * (l16 & 1);
+        const auto four = [&](int rows, int db) __attribute__((always_inline)) {       // rows: a multiple of 8; 8 exchanges by 2
+            const char* x = reinterpret_cast<const char*>(tile) + chunk_from<T, DP>(at, (64 * db) ^ (rows & 8 ? 32 : 0)) + 2 * rows * DP;
+            return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)x);
+        };
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) {
-                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4*)(at + 16 * t * DP + W * ((4 * db + chunk) ^ swap0)));
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4*)(at + (16 * t + 8) * DP + W * ((4 * db + chunk) ^ swap1)));
-                const auto xy = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                const auto xy = __builtin_shufflevector(four(16 * t, db), four(16 * t + 8, db), 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[db] = mfma(__builtin_bit_cast(Frag, xy), w.f[t], acc[db]);
             }
     }
@@ -159,6 +175,7 @@ struct Ops<float> {
     static constexpr int kStep = 8;
     static constexpr int kTile = 32;
     static constexpr int kShift = 0;
+    static constexpr float kSlack = 8.f;
     typedef f32x16 Weights;
 
     static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) {
@@ -170,13 +187,13 @@ struct Ops<float> {
     template <int DP>
     static __device__ __forceinline__ void spread(f32x16* acc, const float* tile, const Weights& w) {
         const int lane = threadIdx.x & 63, half = lane >> 5;
-        const float* at = tile + 4 * half * DP + (lane & 3);
+        const int at = 16 * half * DP + 16 * (((lane >> 2) & 7) ^ (4 * half)) + 4 * (lane & 3);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int row = 8 * (r >> 2) + (r & 3), swap = swizzle<float, DP>(4 * half + row);
+            const int x = (at ^ (16 * (r & 3))) + 4 * (8 * (r >> 2) + (r & 3)) * DP;
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[row * DP + 32 * db + 4 * (((lane >> 2) & 7) ^ swap)], w[r], acc[db], 0, 0, 0);
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(read_at<float>(tile, x + 128 * db), w[r], acc[db], 0, 0, 0);
         }
     }
 };
@@ -196,33 +213,62 @@ struct OwnRow {
             if (row && c < dim) f[s] = *reinterpret_cast<const typename Ops<T>::Frag*>(row + c);
         }
     }
+    __device__ __forceinline__ void negate() {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) f[s] = -f[s];
+    }
     // product with 32 tile rows
     __device__ __forceinline__ f32x16 dot(const T* tile) const {
-        const int lane = threadIdx.x & 63, row = lane & 31, swap = swizzle<T, DP>(row) ^ (lane >> 5);
+        const int lane = threadIdx.x & 63, row = lane & 31;
+        const int at = static_cast<int>(sizeof(T)) * row * DP + 16 * (swizzle<T, DP>(row) ^ (lane >> 5));
         f32x16 acc = {};
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-            acc = Ops<T>::mul(*reinterpret_cast<const typename Ops<T>::Frag*>(tile + row * DP + Ops<T>::W * ((2 * s) ^ swap)), f[s], acc);
+        for (int s = 0; s < kSteps; ++s) acc = Ops<T>::mul(read_at<typename Ops<T>::Frag>(tile, chunk_from<T, DP>(at, 32 * s)), f[s], acc);
         return acc;
     }
 };
 
-// Starts the loads of kTile rows from memory to LDS; they have arrived behind the next arrived(). Rows outside [lo, hi) read
-// the nearest row inside: they are masked, and what memory holds behind a sequence is not looked at. Chunks behind dim
-// read the row's first one: their products with the noughts of an OwnRow are nought, and channels there are not written.
+// Rows of a tensor on their way to tiles in LDS. A tile's loads have one 64-bit address, which the wave keeps in scalar registers, and
+// 32-bit offsets of the lanes, which do not change from tile to tile (the host sees to it that kMaxTile rows span less than 2 GiB).
+// Rows outside [lo, hi) read the nearest row inside: they are masked, and what memory holds behind a sequence is not looked
+// at. Chunks behind dim read the row's first one: their products with the noughts of an OwnRow are nought, and channels there
+// are not written. The loads have arrived behind the next arrived().
 template <typename T, int DP>
-__device__ __forceinline__ void fetch(T* tile, const T* base, int64_t row_stride, int row0, int lo, int hi, int dim) {
-    constexpr int W = Ops<T>::W, kChunks = DP / W, kLoads = Ops<T>::kTile * kChunks / kThreads;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int first = (wave * kLoads + i) * 64, id = first + (threadIdx.x & 63), row = id / kChunks;
-        const int c = W * ((id - row * kChunks) ^ swizzle<T, DP>(row));
-        const int at = min(max(row0 + row, lo), hi - 1);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(base + at * row_stride + (c < dim ? c : 0)),
-                                         (__attribute__((address_space(3))) unsigned*)(tile + first * W), 16, 0, 0);
+struct Fetch {
+    static constexpr int W = Ops<T>::W, kChunks = DP / W, kRows = Ops<T>::kTile, kLoads = kRows * kChunks / kThreads;
+    const char* base;
+    int64_t row_bytes;
+    int lo, hi;
+    unsigned offset[kLoads];
+
+    static __device__ __forceinline__ int piece(int i) {         // of 1 KiB
+        return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kLoads + i;
     }
-}
+    static __device__ __forceinline__ int row_in_tile(int i) { return (piece(i) * 64 + static_cast<int>(threadIdx.x & 63)) / kChunks; }
+    static __device__ __forceinline__ unsigned column(int i, int dim) {
+        const int row = row_in_tile(i), c = W * ((piece(i) * 64 + static_cast<int>(threadIdx.x & 63) - row * kChunks) ^ swizzle<T, DP>(row));
+        return (c < dim ? c : 0) * sizeof(T);
+    }
+    __device__ __forceinline__ void start(const T* tensor, int64_t row_stride, int lo_, int hi_, int dim) {
+        base = reinterpret_cast<const char*>(tensor);
+        row_bytes = row_stride * static_cast<int64_t>(sizeof(T));
+        lo = lo_;
+        hi = hi_;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) offset[i] = static_cast<unsigned>(row_in_tile(i)) * static_cast<unsigned>(row_bytes) + column(i, dim);
+    }
+    __device__ __forceinline__ void load(T* tile, int row0, int dim) const {
+        const char* at = base + row0 * row_bytes;
+        const bool inside = row0 >= lo && row0 + kRows <= hi;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            unsigned o = offset[i];
+            if (!inside) o = static_cast<unsigned>(max(min(row_in_tile(i), hi - 1 - row0), lo - row0)) * static_cast<unsigned>(row_bytes) + column(i, dim);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(at + o),
+                                             (__attribute__((address_space(3))) unsigned*)(tile + piece(i) * 64 * W), 16, 0, 0);
+        }
+    }
+};
 
 // Barrier behind which every wave's fetches are in LDS. __syncthreads() alone does not wait for them: they count as loads from
 // memory, which a workgroup's fence leaves in flight.
@@ -232,32 +278,38 @@ __device__ __forceinline__ void arrived() {
 }
 
 // ---- scores ------------------------------------------------------------------------------------------------------------
-// From q.k to log2(e) u: with a cap, cap log2(e) tanh(scale q.k / cap).
+// From x = |scale| / scale q.k to log2(e) w. Where there is neither cap nor bias that is a product with a constant, which goes into the
+// exponential's argument as exp2(x * mul - maximum), one operation for both; elsewhere log2(e) w is formed first, and mul is 1 there.
 struct Score {
-    float mul, cap, inv;                 // inv: 1 / (cap log2 e), turns the result back into the tanh
-    bool capped;
+    float pre, cap, inv, mul;            // inv: 1 / (cap log2 e), turns the result back into the tanh
+    bool capped, plain;
 
     __device__ __forceinline__ Score(const Dev& a) {
         capped = a.softcap > 0.f;
+        plain = !capped && !a.slopes;
         cap = a.softcap * kLog2e;
         inv = capped ? 1.f / cap : 0.f;
-        mul = capped ? a.scale / a.softcap : a.scale * kLog2e;
+        // at scale 0 a number that makes every score nought and still keeps -infinity (a masked key) what it is
+        pre = fmaxf(fabsf(capped ? a.scale / a.softcap : a.scale * kLog2e), 1e-37f);
+        mul = plain ? pre : 1.f;
     }
+    // x into log2(e) u, where not plain
     template <typename T>
     __device__ __forceinline__ void apply(f32x16& s) const {
+        if (plain) return;
         if (!capped) {
-            s *= mul;
-        } else {
+            s *= pre;
+            return;
+        }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float x = s[r] * mul;
-                if constexpr (__is_same(T, float)) {
-                    s[r] = cap * tanhf(x);
-                } else {
-                    // tanh x = 1 - 2 / (e^2x + 1): off by some 2^-23 of the cap, far below the rounding of 16-bit weights
-                    const float e = exp2_(x * (2.f * kLog2e));
-                    s[r] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(e + 1.f), cap);
-                }
+        for (int r = 0; r < 16; ++r) {
+            const float x = s[r] * pre;
+            if constexpr (__is_same(T, float)) {
+                s[r] = cap * tanhf(x);
+            } else {
+                // tanh x = 1 - 2 / (e^2x + 1): off by some 2^-23 of the cap, far below the rounding of 16-bit weights
+                const float e = exp2_(x * (2.f * kLog2e));
+                s[r] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(e + 1.f), cap);
             }
         }
     }
@@ -271,7 +323,9 @@ struct Score {
 // tile row of register r of this lane half
 __device__ __forceinline__ int reg_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
-bool check_args(const ddpm_span_attention_args& a);              // span_attention_fwd.hip
+// span_attention_fwd.hip
+bool check_args(const ddpm_span_attention_args& a);
+bool fits_tile(const ddpm_span_attention_args& a, const int64_t* stride);      // rows of a tile within 32-bit offsets
 Dev dev_args(const ddpm_span_attention_args& a);
 
 // f(head size as a compile-time constant): dim rounded up to a multiple of 32

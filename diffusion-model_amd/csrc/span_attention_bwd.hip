@@ -90,6 +90,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     OwnRow<T, DP> q, dout;
     q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
     dout.load(real ? static_cast<const T*>(a.dout) + b * a.sdo.batch + i * a.sdo.row + head * a.sdo.head : nullptr, a.dim);
+    if (a.scale < 0.f) q.negate();       // Score counts on a factor that is positive
     float delta = 0.f, stat = -kNoMax;
     {
         OwnRow<T, DP> out;
@@ -111,20 +112,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
 
     const Score score(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
-    const T* k = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
-    const T* v = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
     f32x16 acc[DP / 32] = {};
     float gain = gain_for(0.f), largest = 0.f;
+    Fetch<T, DP> ks, vs;
+    ks.start(static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head, a.sk.row, lo, hi, a.dim);
+    vs.start(static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head, a.sv.row, lo, hi, a.dim);
     if (first < last) {
-        fetch<T, DP>(k_even, k, a.sk.row, first * kTile, lo, hi, a.dim);
-        fetch<T, DP>(v_even, v, a.sv.row, first * kTile, lo, hi, a.dim);
+        ks.load(k_even, first * kTile, a.dim);
+        vs.load(v_even, first * kTile, a.dim);
     }
     const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
         arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
         if (t + 1 < last) {
-            fetch<T, DP>(k_next, k, a.sk.row, j0 + kTile, lo, hi, a.dim);
-            fetch<T, DP>(v_next, v, a.sv.row, j0 + kTile, lo, hi, a.dim);
+            ks.load(k_next, j0 + kTile, a.dim);
+            vs.load(v_next, j0 + kTile, a.dim);
         }
         if (j0 + kTile <= wlo || j0 >= whi) return;
         const bool whole = __all(row.lo <= j0 && row.hi >= j0 + kTile);
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
                 const int j = j0 + 32 * kb + reg_row(e, half);
                 float w = s[e];
                 if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(row.pos - j)), w);
-                float d = exp2_(w - stat) * (dp[e] - delta) * a.scale;
+                float d = exp2_(fmaf(w, score.mul, -stat)) * (dp[e] - delta);
                 if (score.capped) d *= score.slope(s[e]);
                 if (!whole && (j < row.lo || j >= row.hi)) d = 0.f;
                 ds[e] = d;
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
         if (lane == 0) work.largest[(static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave] = largest;
     }
     if (real)
-        write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, kGain ? inverse_gain(gain) : 1.f, a.dim);
+        write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, kGain ? inverse_gain(gain) * a.scale : a.scale, a.dim);
 }
 
 // The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other. A lane holds what one of 64
@@ -245,6 +247,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
     k.load(real ? static_cast<const T*>(a.k) + b * a.sk.batch + j * a.sk.row + kv * a.sk.head : nullptr, a.dim);
     v.load(real ? static_cast<const T*>(a.v) + b * a.sv.batch + j * a.sv.row + kv * a.sv.head : nullptr, a.dim);
 
+    if (a.scale < 0.f) k.negate();       // used in scores alone
     float gain = 1.f;
     if constexpr (kGain) {
         const float* largest = work.largest + (static_cast<int64_t>(b) * a.heads + kv * a.group) * work.groups;
@@ -272,6 +275,9 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
     // the loads of its q and dout, in this order, so that the registers do not have to wait for the tile.
     Row row = no_row();
     float stat = 0.f, delta = 0.f, next_slope = 0.f;
+    Fetch<T, DP> qs, dos;
+    qs.start(static_cast<const T*>(a.q), a.sq.row, 0, a.nq, a.dim);
+    dos.start(static_cast<const T*>(a.dout), a.sdo.row, 0, a.nq, a.dim);
     const auto load = [&](T* q_to, T* do_to) __attribute__((always_inline)) {
         const int head = kv * a.group + tiles.head, i0 = tiles.tile * kTile;
         if (a.slopes) next_slope = a.slopes[head] * kLog2e;
@@ -287,15 +293,17 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
                 delta = work.delta[at];
             }
         }
-        fetch<T, DP>(q_to, static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, a.sq.row, i0, 0, a.nq, a.dim);
-        fetch<T, DP>(do_to, static_cast<const T*>(a.dout) + b * a.sdo.batch + head * a.sdo.head, a.sdo.row, i0, 0, a.nq, a.dim);
+        qs.base = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head);
+        dos.base = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + b * a.sdo.batch + head * a.sdo.head);
+        qs.load(q_to, i0, a.dim);
+        dos.load(do_to, i0, a.dim);
     };
     const auto write_rows = [&](int to) __attribute__((always_inline)) {
         if (threadIdx.x < kTile) {
             lo_tile[to][threadIdx.x] = row.lo;
             hi_tile[to][threadIdx.x] = row.hi;
             pos_tile[to][threadIdx.x] = row.pos;
-            stat_tile[to][threadIdx.x] = stat_of(stat);
+            stat_tile[to][threadIdx.x] = Ops<T>::kShift - stat_of(stat);
             delta_tile[to][threadIdx.x] = delta;
         }
     };
@@ -339,13 +347,13 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
                 const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile[in] + at);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float w = s[4 * x + e] + Ops<T>::kShift - stats[e];
+                    float w = s[4 * x + e];
                     if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(pos_tile[in][at + e] - j)), w);
-                    float y = exp2_(w), d = y * (dp[4 * x + e] - deltas[e]) * (a.scale * kUnshift);
+                    float y = exp2_(fmaf(w, score.mul, stats[e])), d = y * (dp[4 * x + e] - deltas[e]);
                     if (score.capped) d *= score.slope(s[4 * x + e]);
                     if (!whole && (j < lo_tile[in][at + e] || j >= hi_tile[in][at + e])) y = d = 0.f;
                     p[4 * x + e] = y;
-                    ds[4 * x + e] = kGain ? d * gain : d;
+                    ds[4 * x + e] = kGain ? d * (gain * kUnshift) : d;
                 }
             }
             Ops<T>::template spread<DP>(dv, do_now + g * 32 * DP, Ops<T>::pack(p));
@@ -358,7 +366,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
         if (more) step(1, q_odd, do_odd, q_even, do_even);
     }
     if (!real) return;
-    write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, kGain ? inverse_gain(gain) : 1.f, a.dim);
+    write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, kGain ? inverse_gain(gain) * a.scale : a.scale, a.dim);
     write_row<T, DP>(static_cast<T*>(a.dv) + b * a.sdv.batch + j * a.sdv.row + kv * a.sdv.head, dv, kUnshift, a.dim);
 }
 
@@ -389,7 +397,7 @@ bool check_bwd(const ddpm_span_attention_args& a) {
     const int w = a.type == DDPM_F32 ? 4 : 8;
     for (const int64_t* s : {a.dout_stride, a.dq_stride, a.dk_stride, a.dv_stride})
         if (s[0] % w || s[1] % w || s[2] % w) return false;
-    return true;
+    return fits_tile(a, a.q_stride) && fits_tile(a, a.dout_stride);
 }
 
 }  // namespace

@@ -12,6 +12,10 @@ using ddpm::as_stream;
 
 namespace span {
 
+bool fits_tile(const ddpm_span_attention_args& a, const int64_t* stride) {
+    return stride[1] >= 0 && stride[1] < (int64_t(1) << 31) / kMaxTile / (a.type == DDPM_F32 ? 4 : 2);
+}
+
 bool check_args(const ddpm_span_attention_args& a) {
     const int w = a.type == DDPM_F32 ? 4 : 8;
     const auto fits = [&](const int64_t* s) { return s[0] % w == 0 && s[1] % w == 0 && s[2] % w == 0; };
@@ -19,7 +23,7 @@ bool check_args(const ddpm_span_attention_args& a) {
            a.heads >= 1 && a.heads <= 65535 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0 && a.dim >= w &&
            a.dim <= DDPM_SPAN_ATTENTION_MAX_DIM && a.dim % w == 0 && a.nq <= (1 << 30) && a.nk <= (1 << 30) && a.softcap >= 0.f &&
            a.softcap <= 1e30f && a.scale >= -1e30f && a.scale <= 1e30f && fits(a.q_stride) && fits(a.k_stride) && fits(a.v_stride) &&
-           fits(a.out_stride);
+           fits(a.out_stride) && fits_tile(a, a.k_stride) && fits_tile(a, a.v_stride);
 }
 
 Dev dev_args(const ddpm_span_attention_args& a) {
@@ -121,6 +125,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
     }
     OwnRow<T, DP> q;
     q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
+    if (a.scale < 0.f) q.negate();       // Score counts on a factor that is positive
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
@@ -134,21 +139,22 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
 
     const Score score(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
-    const T* k = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
-    const T* v = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
 
     f32x16 acc[DP / 32] = {};
     float top = kNoMax, sum = 0.f;       // of this column: maximum of all its scores, sum of this lane half's weights
+    Fetch<T, DP> ks, vs;
+    ks.start(static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head, a.sk.row, lo, hi, a.dim);
+    vs.start(static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head, a.sv.row, lo, hi, a.dim);
     if (first < last) {
-        fetch<T, DP>(k_even, k, a.sk.row, first * kTile, lo, hi, a.dim);
-        fetch<T, DP>(v_even, v, a.sv.row, first * kTile, lo, hi, a.dim);
+        ks.load(k_even, first * kTile, a.dim);
+        vs.load(v_even, first * kTile, a.dim);
     }
     const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
         arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
         if (t + 1 < last) {
-            fetch<T, DP>(k_next, k, a.sk.row, j0 + kTile, lo, hi, a.dim);
-            fetch<T, DP>(v_next, v, a.sv.row, j0 + kTile, lo, hi, a.dim);
+            ks.load(k_next, j0 + kTile, a.dim);
+            vs.load(v_next, j0 + kTile, a.dim);
         }
         if (j0 + kTile <= wlo || j0 >= whi) return;                 // nothing here for this wave's rows
         f32x16 s[kBlocks];
@@ -178,8 +184,8 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) m = fmaxf(m, s[kb][e]);
-        m = fmaxf(m, other_half(m));
-        if (__any(m > top)) {
+        m = fmaxf(m, other_half(m)) * score.mul;
+        if (__any(m > top + Ops<T>::kSlack)) {
             m = fmaxf(m, top);
             const float f = exp2_(top - m);
             top = m;
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         for (int kb = 0; kb < kBlocks; ++kb) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[kb][e] = exp2_(s[kb][e] + shift);
+                s[kb][e] = exp2_(fmaf(s[kb][e], score.mul, shift));
                 sum += s[kb][e];
             }
             Ops<T>::template spread<DP>(acc, v_now + kb * 32 * DP, Ops<T>::pack(s[kb]));

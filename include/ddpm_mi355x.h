@@ -419,7 +419,8 @@ int ddpm_self_attention_infer(const float* x, int ldx, const float* wqkv_packed,
  * row sees have gradient 0, and what q, k and v hold there does not matter; a value that is not finite at a key that some row sees
  * may reach other rows of that batch entry, as a product with weight nought does.
  * Element (b, n, h, c) of a tensor lies at its base + b*stride[0] + n*stride[1] + h*stride[2] + c. Bases must be 16-byte
- * aligned, and dim and the strides of q, k, v, out and the gradients multiples of 16 bytes (4 fp32, 8 16-bit elements).
+ * aligned, dim and the strides of q, k, v, out and the gradients multiples of 16 bytes (4 fp32, 8 16-bit elements), and the
+ * row strides of k and v (backward: of q and dout too) not negative and below 32 MiB.
  * Arithmetic: fp32 inputs use the fp32 matrix instructions; 16-bit inputs have their weights and score gradients rounded
  * to 16 bits before the second product; scores, softmax statistics and sums are fp32 throughout.
  * Stands beside ddpm_attention_fwd / _bwd (one head, no mask, second-iteration/unet.py:50-61).
