@@ -135,16 +135,24 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
             f32x16 s = q.dot(k_now + kb * 32 * DP);
             const f32x16 dp = dout.dot(v_now + kb * 32 * DP);
             score.apply<T>(s);
-            f32x16 ds;
+            f32x16 ds = s;               // log2(e) w, then p, then ds; the uniform cases stand outside of the loops over elements
+            if (a.slopes) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = j0 + 32 * kb + reg_row(e, half);
-                float w = s[e];
-                if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(row.pos - j)), w);
-                float d = exp2_(fmaf(w, score.mul, -stat)) * (dp[e] - delta);
-                if (score.capped) d *= score.slope(s[e]);
-                if (!whole && (j < row.lo || j >= row.hi)) d = 0.f;
-                ds[e] = d;
+                for (int e = 0; e < 16; ++e)
+                    ds[e] = fmaf(-slope, fabsf(static_cast<float>(row.pos - (j0 + 32 * kb + reg_row(e, half)))), ds[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ds[e] = exp2_(fmaf(ds[e], score.mul, -stat)) * (dp[e] - delta);
+            if (score.capped) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ds[e] *= score.slope(s[e]);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = j0 + 32 * kb + reg_row(e, half);
+                    if (j < row.lo || j >= row.hi) ds[e] = 0.f;
+                }
             }
             if constexpr (kGain) {
                 float m = 0.f;
@@ -339,23 +347,34 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
             f32x16 s = k.dot(q_now + g * 32 * DP);
             const f32x16 dp = v.dot(do_now + g * 32 * DP);
             score.apply<T>(s);
-            f32x16 p, ds;
+            f32x16 p = s, ds;            // log2(e) w, then p; the uniform cases stand outside of the loops over elements
+            if (a.slopes) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    p[e] = fmaf(-slope, fabsf(static_cast<float>(pos_tile[in][32 * g + reg_row(e, half)] - j)), p[e]);
+            }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const int at = 32 * g + 8 * x + 4 * half;              // four rows
-                const f32x4 stats = *reinterpret_cast<const f32x4*>(stat_tile[in] + at);
-                const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile[in] + at);
+                const f32x4 stats = *reinterpret_cast<const f32x4*>(stat_tile[in] + 32 * g + 8 * x + 4 * half);       // of four rows
+                const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile[in] + 32 * g + 8 * x + 4 * half);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float w = s[4 * x + e];
-                    if (a.slopes) w = fmaf(-slope, fabsf(static_cast<float>(pos_tile[in][at + e] - j)), w);
-                    float y = exp2_(fmaf(w, score.mul, stats[e])), d = y * (dp[4 * x + e] - deltas[e]);
-                    if (score.capped) d *= score.slope(s[4 * x + e]);
-                    if (!whole && (j < lo_tile[in][at + e] || j >= hi_tile[in][at + e])) y = d = 0.f;
-                    p[4 * x + e] = y;
-                    ds[4 * x + e] = kGain ? d * (gain * kUnshift) : d;
+                    p[4 * x + e] = exp2_(fmaf(p[4 * x + e], score.mul, stats[e]));
+                    ds[4 * x + e] = p[4 * x + e] * (dp[4 * x + e] - deltas[e]);
                 }
             }
+            if (score.capped) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ds[e] *= score.slope(s[e]);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int at = 32 * g + reg_row(e, half);
+                    if (j < lo_tile[in][at] || j >= hi_tile[in][at]) p[e] = ds[e] = 0.f;
+                }
+            }
+            if constexpr (kGain) ds *= gain * kUnshift;
             Ops<T>::template spread<DP>(dv, do_now + g * 32 * DP, Ops<T>::pack(p));
             Ops<T>::template spread<DP>(dk, q_now + g * 32 * DP, Ops<T>::pack(ds));
         }
