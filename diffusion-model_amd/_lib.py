@@ -44,7 +44,7 @@ class RotaryArgs(C.Structure):
 class SpanAttentionArgs(C.Structure):
     _fields_ = [(n, I32) for n in ("type", "batch", "nq", "nk", "heads", "kv_heads", "dim", "causal")] + \
                [("scale", F32), ("softcap", F32), ("slopes", P), ("spans", P), ("positions", P), ("span_batch_stride", I64),
-                ("position_batch_stride", I64), ("q", P), ("k", P), ("v", P), ("out", P), ("lse", P)] + \
+                ("position_batch_stride", I64), ("q", P), ("k", P), ("v", P), ("out", P), ("out_low", P), ("lse", P)] + \
                [(n, I64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
                [(n, P) for n in ("dout", "dq", "dk", "dv")] + \
                [(n, I64 * 3) for n in ("dout_stride", "dq_stride", "dk_stride", "dv_stride")]

@@ -74,7 +74,7 @@ def _put(a, name, x, stride):
     getattr(a, stride)[:] = [s if n > 1 else 0 for n, s in zip(x.shape[:3], x.stride())]
 
 
-def _arguments(q, k, v, out, lse, how):
+def _arguments(q, k, v, out, low, lse, how):
     scale, softcap, slopes, spans, positions, causal = how
     a = SpanAttentionArgs()
     a.type = _TYPES[q.dtype][0]
@@ -91,6 +91,8 @@ def _arguments(q, k, v, out, lse, how):
     _put(a, "k", k, "k_stride")
     _put(a, "v", v, "v_stride")
     _put(a, "out", out, "out_stride")
+    if low is not None:
+        a.out_low = low.data_ptr()
     if lse is not None:
         a.lse = lse.data_ptr()
     return a
@@ -102,21 +104,22 @@ def _run(entry, a, device):
     call(entry, C.byref(a), C.c_void_p(workspace.data_ptr() if size > 0 else None), C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
 
 
-def _forward(q, k, v, how, with_lse):
+def _forward(q, k, v, how, with_lse, with_low=False):
     width = _TYPES[q.dtype][1]
     q, k, v = (_fit(x, width) for x in (q, k, v))
     with torch.cuda.device(q.device):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if with_lse else None
-        _run("ddpm_span_attention_fwd", _arguments(q, k, v, out, lse, how), q.device)
-    return q, k, v, out, lse
+        low = torch.empty_like(out) if with_low and q.dtype != torch.float32 else None
+        _run("ddpm_span_attention_fwd", _arguments(q, k, v, out, low, lse, how), q.device)
+    return q, k, v, out, low, lse
 
 
 class _SpanAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, softcap, slopes, spans, positions, causal):
-        q, k, v, out, lse = _forward(q, k, v, (scale, softcap, slopes, spans, positions, causal), True)
-        ctx.save_for_backward(q, k, v, out, lse, slopes, spans, positions)
+        q, k, v, out, low, lse = _forward(q, k, v, (scale, softcap, slopes, spans, positions, causal), True, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, slopes, spans, positions)
         ctx.how = scale, softcap, causal
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -127,12 +130,12 @@ class _SpanAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return (None,) * 9
-        q, k, v, out, lse, slopes, spans, positions = ctx.saved_tensors
+        q, k, v, out, low, lse, slopes, spans, positions = ctx.saved_tensors
         scale, softcap, causal = ctx.how
         dout = _fit(dout, _TYPES[q.dtype][1])
         with torch.cuda.device(q.device):
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-            a = _arguments(q, k, v, out, lse, (scale, softcap, slopes, spans, positions, causal))
+            a = _arguments(q, k, v, out, low, lse, (scale, softcap, slopes, spans, positions, causal))
             _put(a, "dout", dout, "dout_stride")
             _put(a, "dq", dq, "dq_stride")
             _put(a, "dk", dk, "dk_stride")
@@ -192,7 +195,7 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v)):
         out, lse = _SpanAttention.apply(q, k, v, scale, float(softcap), slopes, spans, positions, bool(causal))
     else:
-        *_, out, lse = _forward(q, k, v, (scale, float(softcap), slopes, spans, positions, bool(causal)), return_lse)
+        _, _, _, out, _, lse = _forward(q, k, v, (scale, float(softcap), slopes, spans, positions, bool(causal)), return_lse)
     if spare:
         out = out[..., :dim].contiguous()
     return (out, lse) if return_lse else out

@@ -93,12 +93,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     if (a.scale < 0.f) q.negate();       // Score counts on a factor that is positive
     float delta = 0.f, stat = -kNoMax;
     {
-        OwnRow<T, DP> out;
-        out.load(real ? static_cast<const T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head : nullptr, a.dim);
+        const int64_t mine = b * a.so.batch + i * a.so.row + head * a.so.head;
+        OwnRow<T, DP> out, low;
+        out.load(real ? static_cast<const T*>(a.out) + mine : nullptr, a.dim);
+        low.load(real && sizeof(T) == 2 && a.out_low ? static_cast<const T*>(a.out_low) + mine : nullptr, a.dim);
 #pragma unroll
         for (int s = 0; s < OwnRow<T, DP>::kSteps; ++s)
 #pragma unroll
-            for (int e = 0; e < Ops<T>::W; ++e) delta = fmaf(static_cast<float>(dout.f[s][e]), static_cast<float>(out.f[s][e]), delta);
+            for (int e = 0; e < Ops<T>::W; ++e)
+                delta = fmaf(static_cast<float>(dout.f[s][e]), static_cast<float>(out.f[s][e]) + static_cast<float>(low.f[s][e]), delta);
         delta += other_half(delta);
     }
     if (real) {
@@ -434,7 +437,7 @@ extern "C" int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* 
     if (a->batch == 0) return DDPM_OK;
     DDPM_REQUIRE(a->nq == 0 || (a->q && a->out && a->lse && a->dout && a->dq));
     DDPM_REQUIRE(a->nk == 0 || (a->k && a->v && a->dk && a->dv));
-    for (const void* p : {a->q, a->k, a->v, static_cast<const void*>(a->out), a->dout, static_cast<const void*>(a->dq),
+    for (const void* p : {a->q, a->k, a->v, static_cast<const void*>(a->out), static_cast<const void*>(a->out_low), a->dout, static_cast<const void*>(a->dq),
                           static_cast<const void*>(a->dk), static_cast<const void*>(a->dv), static_cast<const void*>(workspace)})
         DDPM_REQUIRE(ddpm::aligned16(p));
     DDPM_REQUIRE(a->nq == 0 || workspace);

@@ -46,6 +46,7 @@ Dev dev_args(const ddpm_span_attention_args& a) {
     d.k = a.k;
     d.v = a.v;
     d.out = a.out;
+    d.out_low = a.out_low;
     d.lse = a.lse;
     d.sq = strides(a.q_stride);
     d.sk = strides(a.k_stride);
@@ -231,17 +232,14 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
     }
     if (a.lse && half == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top - Ops<T>::kShift + log2f(sum)) * kLn2;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* out = static_cast<T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head;
-    typedef T T4 __attribute__((ext_vector_type(4)));
+    const int64_t out = b * a.so.batch + i * a.so.row + head * a.so.head;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d = 32 * db + 8 * g + 4 * half;
-            T4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[db][4 * g + e] * inv);
-            if (d < a.dim) *reinterpret_cast<T4*>(out + d) = o;
+            const float o[4] = {acc[db][4 * g] * inv, acc[db][4 * g + 1] * inv, acc[db][4 * g + 2] * inv, acc[db][4 * g + 3] * inv};
+            if (d < a.dim) write_out<T>(a, out + d, o);
         }
 }
 
@@ -297,11 +295,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Dev a, const Parts part
 #pragma unroll
     for (int g = 1; g < 8; ++g) acc += group_acc[g][threadIdx.x];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[e] * inv);
-    *reinterpret_cast<T4*>(static_cast<T*>(a.out) + b * a.so.batch + i * a.so.row + head * a.so.head + c) = o;
+    const float o[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    write_out<T>(a, b * a.so.batch + i * a.so.row + head * a.so.head + c, o);
 }
 
 template <typename T>
@@ -335,7 +330,7 @@ extern "C" int ddpm_span_attention_fwd(const ddpm_span_attention_args* a, void* 
     DDPM_REQUIRE(a && span::check_args(*a));
     if (a->batch == 0 || a->nq == 0) return DDPM_OK;
     DDPM_REQUIRE(a->q && a->out && (a->nk == 0 || (a->k && a->v)));
-    DDPM_REQUIRE(ddpm::aligned16(a->q) && ddpm::aligned16(a->k) && ddpm::aligned16(a->v) && ddpm::aligned16(a->out));
+    DDPM_REQUIRE(ddpm::aligned16(a->q) && ddpm::aligned16(a->k) && ddpm::aligned16(a->v) && ddpm::aligned16(a->out) && ddpm::aligned16(a->out_low));
     const Plan plan = plan_of(*a);
     DDPM_REQUIRE(plan.splits == 1 || (workspace && ddpm::aligned16(workspace)));
     if (a->type == DDPM_F32)

@@ -437,9 +437,11 @@ typedef struct ddpm_span_attention_args {
     int64_t span_batch_stride, position_batch_stride;   /* elements; 0 = shared by the batch */
     const void *q, *k, *v;
     void* out;
+    void* out_low;                   /* like out, 16-bit types: what out's rounding left, written by the forward call and read by the
+                                        backward one; NULL: score gradients take out as it is, and are less exact */
     float* lse;                      /* [batch][heads][nq]; forward: may be NULL */
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* elements: batch, row, head */
-    /* the backward call; out and lse are the forward's */
+    /* the backward call; out, out_low and lse are the forward's */
     const void* dout;
     void *dq, *dk, *dv;
     int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
