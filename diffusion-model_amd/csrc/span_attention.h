@@ -111,6 +111,15 @@ __device__ __forceinline__ int chunk_from(int at, int delta) {
     return (at ^ (delta & (power - 1))) + (delta & ~(power - 1));
 }
 
+// The offsets of a product differ by constants from one, but an exclusive or is no offset that an instruction has room for: left
+// alone (FRESH false), the compiler computes all of them ahead of the loop and keeps them in registers, 16 and more. Where those are
+// wanted for something else they are computed as they are used.
+template <bool FRESH>
+__device__ __forceinline__ int offset(int at) {
+    if (FRESH) asm volatile("" : "+v"(at));
+    return at;
+}
+
 template <typename V, typename T>
 __device__ __forceinline__ V read_at(const T* tile, int at) {
     return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(tile) + at);
@@ -146,13 +155,13 @@ struct Ops {                             // bf16, fp16
         return w;
     }
     // acc[db] += over 32 tile rows; `tile` points at the first of them
-    template <int DP>
+    template <int DP, bool FRESH = false>
     static __device__ __forceinline__ void spread(f32x16* acc, const T* tile, const Weights& w) {
         // The transposing read gives lane l of 16 the column l of a 4 x 16 block whose rows four lanes each point at: rows
         // 4 h ... 4 h + 3 (and 8 further) are the ones whose weights this lane half holds.
         const int lane = threadIdx.x & 63, l16 = lane & 15, row = 4 * (lane >> 5) + (l16 >> 2);
         const int chunk = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
-        const int at = 2 * row * DP + 16 * (chunk ^ swizzle<T, DP>(row)) + 8 * (l16 & 1);
+        const int at = offset<FRESH>(2 * row * DP + 16 * (chunk ^ swizzle<T, DP>(row)) + 8 * (l16 & 1));
         const auto four = [&](int rows, int db) __attribute__((always_inline)) {       // rows: a multiple of 8; 8 exchanges by 2
             const char* x = reinterpret_cast<const char*>(tile) + chunk_from<T, DP>(at, (64 * db) ^ (rows & 8 ? 32 : 0)) + 2 * rows * DP;
             return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)x);
@@ -184,10 +193,10 @@ struct Ops<float> {
         return c;
     }
     static __device__ __forceinline__ Weights pack(const f32x16& p) { return p; }
-    template <int DP>
+    template <int DP, bool FRESH = false>
     static __device__ __forceinline__ void spread(f32x16* acc, const float* tile, const Weights& w) {
         const int lane = threadIdx.x & 63, half = lane >> 5;
-        const int at = 16 * half * DP + 16 * (((lane >> 2) & 7) ^ (4 * half)) + 4 * (lane & 3);
+        const int at = offset<FRESH>(16 * half * DP + 16 * (((lane >> 2) & 7) ^ (4 * half)) + 4 * (lane & 3));
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int x = (at ^ (16 * (r & 3))) + 4 * (8 * (r >> 2) + (r & 3)) * DP;
@@ -217,10 +226,11 @@ struct OwnRow {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) f[s] = -f[s];
     }
-    // product with 32 tile rows
+    // product with 32 tile rows; like it with the own rows, 32 of a wave, in LDS too
+    template <bool FRESH = false>
     __device__ __forceinline__ f32x16 dot(const T* tile) const {
         const int lane = threadIdx.x & 63, row = lane & 31;
-        const int at = static_cast<int>(sizeof(T)) * row * DP + 16 * (swizzle<T, DP>(row) ^ (lane >> 5));
+        const int at = offset<FRESH>(static_cast<int>(sizeof(T)) * row * DP + 16 * (swizzle<T, DP>(row) ^ (lane >> 5)));
         f32x16 acc = {};
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) acc = Ops<T>::mul(read_at<typename Ops<T>::Frag>(tile, chunk_from<T, DP>(at, 32 * s)), f[s], acc);
@@ -228,22 +238,35 @@ struct OwnRow {
     }
 };
 
+template <typename T, int DP, bool FRESH = false>
+__device__ __forceinline__ f32x16 dot_from_lds(const T* tile, const T* own) {
+    const int lane = threadIdx.x & 63, row = lane & 31;
+    const int at = offset<FRESH>(static_cast<int>(sizeof(T)) * row * DP + 16 * (swizzle<T, DP>(row) ^ (lane >> 5)));
+    f32x16 acc = {};
+#pragma unroll
+    for (int s = 0; s < DP / Ops<T>::kStep; ++s) {
+        acc = Ops<T>::mul(read_at<typename Ops<T>::Frag>(tile, chunk_from<T, DP>(at, 32 * s)),
+                          read_at<typename Ops<T>::Frag>(own, chunk_from<T, DP>(at, 32 * s)), acc);
+    }
+    return acc;
+}
+
 // Rows of a tensor on their way to tiles in LDS. A tile's loads have one 64-bit address, which the wave keeps in scalar registers, and
 // 32-bit offsets of the lanes, which do not change from tile to tile (the host sees to it that kMaxTile rows span less than 2 GiB).
 // Rows outside [lo, hi) read the nearest row inside: they are masked, and what memory holds behind a sequence is not looked
 // at. Chunks behind dim read the row's first one: their products with the noughts of an OwnRow are nought, and channels there
 // are not written. The loads have arrived behind the next arrived().
-template <typename T, int DP>
+template <typename T, int DP, int ROWS = Ops<T>::kTile>
 struct Fetch {
-    static constexpr int W = Ops<T>::W, kChunks = DP / W, kRows = Ops<T>::kTile, kLoads = kRows * kChunks / kThreads;
+    static constexpr int W = Ops<T>::W, kChunks = DP / W, kRows = ROWS, kPieces = kRows * kChunks / 64, kWaves = kThreads / 64;
+    static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves;      // pieces of 1 KiB, in turn for the waves
+    static_assert(kRows * kChunks % 64 == 0, "whole pieces");
     const char* base;
     int64_t row_bytes;
     int lo, hi;
     unsigned offset[kLoads];
 
-    static __device__ __forceinline__ int piece(int i) {         // of 1 KiB
-        return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kLoads + i;
-    }
+    static __device__ __forceinline__ int piece(int i) { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + i * kWaves; }
     static __device__ __forceinline__ int row_in_tile(int i) { return (piece(i) * 64 + static_cast<int>(threadIdx.x & 63)) / kChunks; }
     static __device__ __forceinline__ unsigned column(int i, int dim) {
         const int row = row_in_tile(i), c = W * ((piece(i) * 64 + static_cast<int>(threadIdx.x & 63) - row * kChunks) ^ swizzle<T, DP>(row));
@@ -262,6 +285,7 @@ struct Fetch {
         const bool inside = row0 >= lo && row0 + kRows <= hi;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
+            if (kPieces % kWaves && piece(i) >= kPieces) break;
             unsigned o = offset[i];
             if (!inside) o = static_cast<unsigned>(max(min(row_in_tile(i), hi - 1 - row0), lo - row0)) * static_cast<unsigned>(row_bytes) + column(i, dim);
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(at + o),
@@ -270,11 +294,37 @@ struct Fetch {
     }
 };
 
+// 64 lanes' words of 4 bytes from memory to LDS, like a Fetch.
+__device__ __forceinline__ void fetch_words(void* to, const void* from) {
+    const unsigned lane = 4 * (threadIdx.x & 63);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(static_cast<const char*>(from) + lane),
+                                     (__attribute__((address_space(3))) unsigned*)to, 4, 0, 0);
+}
+
 // Barrier behind which every wave's fetches are in LDS. __syncthreads() alone does not wait for them: they count as loads from
 // memory, which a workgroup's fence leaves in flight.
 __device__ __forceinline__ void arrived() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+}
+
+// Waits until matrix instructions have written x. The compiler inserts these waits itself, but its search for the instruction that
+// wrote a register, going back over a join of branches, may follow the long way round to it alone and find that enough time has
+// passed: a read behind `products; branch around something; join` has met the registers of before. Between products and the
+// next branch the wait is therefore written out: 18 states behind the fp32 instruction, 12 behind the 16-bit ones.
+template <typename T>
+__device__ __forceinline__ void settle(f32x16& x) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("s_nop 15\n\ts_nop 1" : "+v"(x));
+    else
+        asm volatile("s_nop 11" : "+v"(x));
+}
+template <typename T>
+__device__ __forceinline__ void settle(f32x16& x, f32x16& y) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("s_nop 15\n\ts_nop 1" : "+v"(x), "+v"(y));
+    else
+        asm volatile("s_nop 11" : "+v"(x), "+v"(y));
 }
 
 // ---- scores ------------------------------------------------------------------------------------------------------------

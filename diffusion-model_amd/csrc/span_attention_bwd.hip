@@ -20,10 +20,13 @@ struct Seen {
     int lo, hi, all_lo, all_hi;
 };
 
+// What the dq kernel leaves for the other one, in groups of 32 rows.
 struct Work {
-    float* delta;                        // D: [batch][heads][nq]
-    Seen* seen;                          // [batch][groups], groups of 32 rows
-    float* largest;                      // fp16: largest |ds| of the rows of a group: [batch][heads][groups]
+    Seen* seen;                          // [batch][groups]
+    int* spans;                          // [batch][groups][lo of 32 rows | hi]
+    int* positions;                      // [batch][groups][32, and 32 unused]
+    float* stats;                        // [batch][heads][groups][-lse in units of log 2 plus kShift | D]
+    float* largest;                      // fp16: largest |ds| of a group: [batch][heads][groups]
     int groups;
 };
 
@@ -42,7 +45,7 @@ __device__ __forceinline__ float inverse_gain(float gain) {
 __device__ __forceinline__ float stat_of(float lse) { return lse == -INFINITY ? -kNoMax : lse * kLog2e; }
 
 template <typename T, int DP>
-__device__ __forceinline__ void write_row(T* out, const f32x16* acc, float f, int dim) {
+__device__ __forceinline__ void write_row(T* out, const f32x16* acc, float f, int dim) {      // acc has settled
     typedef T T4 __attribute__((ext_vector_type(4)));
     const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
@@ -73,6 +76,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     const Row row = real ? row_of(a, b, i) : no_row();
     int wlo = row.lo, whi = row.hi;
     join_rows(wlo, whi);
+    const int64_t group = static_cast<int64_t>(b) * work.groups + block * 4 + wave;
     if (head == 0) {
         int alo = row.lo, ahi = row.hi;
 #pragma unroll
@@ -80,7 +84,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
             alo = max(alo, __shfl_xor(alo, d));
             ahi = min(ahi, __shfl_xor(ahi, d));
         }
-        if (lane == 0) work.seen[static_cast<int64_t>(b) * work.groups + block * 4 + wave] = {wlo, whi, alo, ahi};
+        if (lane == 0) work.seen[group] = {wlo, whi, alo, ahi};
+        work.spans[64 * group + lane] = half ? row.hi : row.lo;
+        work.positions[64 * group + lane] = row.pos;
     }
     if (lane == 0) {
         bounds[0][wave] = wlo;
@@ -104,10 +110,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
                 delta = fmaf(static_cast<float>(dout.f[s][e]), static_cast<float>(out.f[s][e]) + static_cast<float>(low.f[s][e]), delta);
         delta += other_half(delta);
     }
-    if (real) {
-        stat = stat_of(a.lse[at]);
-        if (half == 0) work.delta[at] = delta;
-    }
+    if (real) stat = stat_of(a.lse[at]);
+    work.stats[64 * ((static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave) + lane] = half ? delta : Ops<T>::kShift - stat;
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
@@ -136,20 +140,22 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
 #pragma unroll
         for (int kb = 0; kb < kBlocks; ++kb) {
             f32x16 s = q.dot(k_now + kb * 32 * DP);
-            const f32x16 dp = dout.dot(v_now + kb * 32 * DP);
+            f32x16 ds = dout.dot(v_now + kb * 32 * DP);
+            settle<T>(s, ds);
             score.apply<T>(s);
-            f32x16 ds = s;               // log2(e) w, then p, then ds; the uniform cases stand outside of the loops over elements
-            if (a.slopes) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    ds[e] = fmaf(-slope, fabsf(static_cast<float>(row.pos - (j0 + 32 * kb + reg_row(e, half)))), ds[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) ds[e] = exp2_(fmaf(ds[e], score.mul, -stat)) * (dp[e] - delta);
+            // s becomes p, dp becomes ds, in place; what is the same for the whole wave stands outside of the loops over elements
+            ds -= delta;
             if (score.capped) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) ds[e] *= score.slope(s[e]);
             }
+            if (a.slopes) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[e] = fmaf(-slope, fabsf(static_cast<float>(row.pos - (j0 + 32 * kb + reg_row(e, half)))), s[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ds[e] *= exp2_(fmaf(s[e], score.mul, -stat));
             if (!whole) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -183,19 +189,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
         for (int d = 16; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
         if (lane == 0) work.largest[(static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave] = largest;
     }
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) settle<T>(acc[db]);
     if (real)
         write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, kGain ? inverse_gain(gain) * a.scale : a.scale, a.dim);
 }
 
-// The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other. A lane holds what one of 64
-// tiles sees, so that going on needs no memory (a load behind the fetches of a tile could only arrive after them).
+// The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other. What a tile sees comes through
+// scalar loads: a vector load behind the fetches of a tile could only arrive after them.
 template <int GROUPS>                    // groups of 32 rows in a tile
 struct Tiles {
+    typedef const __attribute__((address_space(4))) Seen* Scalar;
     const Seen* seen;
     int groups, tiles, heads, begin, end;
-    int base;                            // 64 tiles from `base` on are in `mask` and `mine`
+    int base;                            // 64 tiles from `base` on are in `mask`
     unsigned long long mask;
-    Seen mine[GROUPS];
     // the current one
     int head, tile;
     Seen now[GROUPS];
@@ -204,11 +212,8 @@ struct Tiles {
         const int t = base + (threadIdx.x & 63);
         bool any = false;
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            mine[g] = {INT32_MAX, 0, INT32_MAX, 0};
-            if (t * GROUPS + g < groups) mine[g] = seen[t * GROUPS + g];
-            any |= mine[g].lo < end && mine[g].hi > begin;
-        }
+        for (int g = 0; g < GROUPS; ++g)
+            if (t * GROUPS + g < groups) any |= seen[t * GROUPS + g].lo < end && seen[t * GROUPS + g].hi > begin;
         mask = __ballot(any);
     }
     __device__ __forceinline__ void start() {
@@ -225,38 +230,46 @@ struct Tiles {
             }
             look();
         }
-        const int lane = __builtin_ctzll(mask);
+        tile = base + __builtin_ctzll(mask);
         mask &= mask - 1;
-        tile = base + lane;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            now[g].lo = __builtin_amdgcn_readlane(mine[g].lo, lane);
-            now[g].hi = __builtin_amdgcn_readlane(mine[g].hi, lane);
-            now[g].all_lo = __builtin_amdgcn_readlane(mine[g].all_lo, lane);
-            now[g].all_hi = __builtin_amdgcn_readlane(mine[g].all_hi, lane);
+            const Scalar s = (Scalar)(seen + tile * GROUPS + g);
+            now[g] = {s->lo, s->hi, s->all_lo, s->all_hi};
         }
         return true;
     }
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const Dev a, const Work work) {
-    constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void dkv_kernel(const Dev a, const Work work) {
+#ifndef VL
+#define VL 64
+#endif
+    constexpr bool kLdsV = sizeof(T) == 2 && DP > VL, kFresh = kLdsV && DP > 96;
+    constexpr int kTile = kLdsV ? 32 : Ops<T>::kTile, kBlocks = kTile / 32;
+    __shared__ __attribute__((aligned(1024))) T v_rows[kLdsV ? kRows * DP : 1];
     constexpr bool kGain = __is_same(T, _Float16);
     constexpr float kUnshift = 1.f / (1 << Ops<T>::kShift);
     __shared__ __attribute__((aligned(1024))) T q_even[kTile * DP], q_odd[kTile * DP], do_even[kTile * DP], do_odd[kTile * DP];
-    __shared__ __attribute__((aligned(16))) float stat_tile[2][kTile], delta_tile[2][kTile];
-    __shared__ __attribute__((aligned(16))) int lo_tile[2][kTile], hi_tile[2][kTile], pos_tile[2][kTile];
+    __shared__ __attribute__((aligned(256))) float stats_even[64 * kBlocks], stats_odd[64 * kBlocks];
+    __shared__ __attribute__((aligned(256))) int spans_even[64 * kBlocks], spans_odd[64 * kBlocks], pos_even[64 * kBlocks], pos_odd[64 * kBlocks];
     __shared__ float wave_max[4];
 
     const dim3 id = ddpm::xcd_block();
     const int kv = id.y, b = id.z;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int begin = id.x * kRows, w0 = begin + wave * 32, j = w0 + (lane & 31);   // keys of the workgroup, the wave, the lane
     const bool real = j < a.nk;
     OwnRow<T, DP> k, v;
     k.load(real ? static_cast<const T*>(a.k) + b * a.sk.batch + j * a.sk.row + kv * a.sk.head : nullptr, a.dim);
-    v.load(real ? static_cast<const T*>(a.v) + b * a.sv.batch + j * a.sv.row + kv * a.sv.head : nullptr, a.dim);
+    if constexpr (kLdsV) {
+        Fetch<T, DP, kRows> vs;
+        vs.start(static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head, a.sv.row, 0, a.nk, a.dim);
+        vs.load(v_rows, begin, a.dim);
+    } else {
+        v.load(real ? static_cast<const T*>(a.v) + b * a.sv.batch + j * a.sv.row + kv * a.sv.head : nullptr, a.dim);
+    }
 
     if (a.scale < 0.f) k.negate();       // used in scores alone
     float gain = 1.f;
@@ -282,51 +295,37 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
     tiles.end = min(begin + kRows, a.nk);
     tiles.start();
 
-    // Of the tile that `tiles` stands at: what its rows see, their lse and their D, into registers and then (write_rows) into LDS, and
-    // the loads of its q and dout, in this order, so that the registers do not have to wait for the tile.
-    Row row = no_row();
-    float stat = 0.f, delta = 0.f, next_slope = 0.f;
-    Fetch<T, DP> qs, dos;
+    Fetch<T, DP, kTile> qs, dos;
     qs.start(static_cast<const T*>(a.q), a.sq.row, 0, a.nq, a.dim);
     dos.start(static_cast<const T*>(a.dout), a.sdo.row, 0, a.nq, a.dim);
-    const auto load = [&](T* q_to, T* do_to) __attribute__((always_inline)) {
-        const int head = kv * a.group + tiles.head, i0 = tiles.tile * kTile;
-        if (a.slopes) next_slope = a.slopes[head] * kLog2e;
-        if (threadIdx.x < kTile) {
-            const int i = i0 + threadIdx.x;
-            row = no_row();
-            stat = -kNoMax;
-            delta = 0.f;
-            if (i < a.nq) {
-                const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
-                row = row_of(a, b, i);
-                stat = a.lse[at];
-                delta = work.delta[at];
-            }
-        }
+    // starts the loads of the tile that `tiles` stands at, and of what the other kernel left about its rows
+    const auto load = [&](T* q_to, T* do_to, float* stats_to, int* spans_to, int* pos_to) __attribute__((always_inline)) {
+        const int head = kv * a.group + tiles.head;
         qs.base = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head);
         dos.base = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + b * a.sdo.batch + head * a.sdo.head);
-        qs.load(q_to, i0, a.dim);
-        dos.load(do_to, i0, a.dim);
-    };
-    const auto write_rows = [&](int to) __attribute__((always_inline)) {
-        if (threadIdx.x < kTile) {
-            lo_tile[to][threadIdx.x] = row.lo;
-            hi_tile[to][threadIdx.x] = row.hi;
-            pos_tile[to][threadIdx.x] = row.pos;
-            stat_tile[to][threadIdx.x] = Ops<T>::kShift - stat_of(stat);
-            delta_tile[to][threadIdx.x] = delta;
+        qs.load(q_to, tiles.tile * kTile, a.dim);
+        dos.load(do_to, tiles.tile * kTile, a.dim);
+        const int group = tiles.tile * kBlocks + wave;
+        if (wave < kBlocks) {
+            fetch_words(stats_to + 64 * wave, work.stats + 64 * ((static_cast<int64_t>(b) * a.heads + head) * work.groups + group));
+            fetch_words(spans_to + 64 * wave, work.spans + 64 * (static_cast<int64_t>(b) * work.groups + group));
+            if (a.slopes) fetch_words(pos_to + 64 * wave, work.positions + 64 * (static_cast<int64_t>(b) * work.groups + group));
         }
     };
 
+    if constexpr (kLdsV)
+        if (a.dim < DP) {                // noughts behind dim, as in an OwnRow: both sides of this product come from LDS
+            arrived();
+            constexpr int W = Ops<T>::W, kChunks = DP / W;
+            for (int x = threadIdx.x; x < kRows * kChunks; x += kThreads)
+                if (W * ((x % kChunks) ^ swizzle<T, DP>(x / kChunks)) >= a.dim) reinterpret_cast<typename Ops<T>::Frag*>(v_rows)[x] = {};
+        }
     bool more = tiles.next();
-    if (more) {
-        load(q_even, do_even);
-        write_rows(0);
-    }
-    const auto step = [&](int in, T* q_now, T* do_now, T* q_next, T* do_next) __attribute__((always_inline)) {
+    if (more) load(q_even, do_even, stats_even, spans_even, pos_even);
+    const auto step = [&](T* q_now, T* do_now, const float* stats_now, const int* spans_now, const int* pos_now, T* q_next, T* do_next,
+                          float* stats_next, int* spans_next, int* pos_next) __attribute__((always_inline)) {
         arrived();                       // this tile is here, the one before is done with
-        const float slope = next_slope;
+        const int head = kv * a.group + tiles.head;
         Seen now[kBlocks];
         bool all = true;                 // does every row see some key?
 #pragma unroll
@@ -334,12 +333,13 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
             now[g] = tiles.now[g];
             all &= now[g].all_lo != INT32_MAX;
         }
+        const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
         more = tiles.next();
-        if (more) load(q_next, do_next);
+        if (more) load(q_next, do_next, stats_next, spans_next, pos_next);
         if (!all) {                      // what q and dout hold in a row that sees none does not matter: noughts
             constexpr int kChunks = DP / Ops<T>::W;
             for (int x = threadIdx.x; x < kTile * kChunks; x += kThreads)
-                if (hi_tile[in][x / kChunks] == 0)
+                if (spans_now[64 * (x / kChunks / 32) + 32 + x / kChunks % 32] == 0)
                     reinterpret_cast<typename Ops<T>::Frag*>(q_now)[x] = reinterpret_cast<typename Ops<T>::Frag*>(do_now)[x] = {};
             __syncthreads();
         }
@@ -347,46 +347,60 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
         for (int g = 0; g < kBlocks; ++g) {
             if (now[g].lo >= w0 + 32 || now[g].hi <= w0) continue;
             const bool whole = now[g].all_lo <= w0 && now[g].all_hi >= w0 + 32;
-            f32x16 s = k.dot(q_now + g * 32 * DP);
-            const f32x16 dp = v.dot(do_now + g * 32 * DP);
+            f32x16 s = k.template dot<kFresh>(q_now + g * 32 * DP);
+            if (kFresh) __builtin_amdgcn_sched_barrier(0);
+            f32x16 ds;
+            if constexpr (kLdsV)
+                ds = dot_from_lds<T, DP, kFresh>(do_now + g * 32 * DP, v_rows + wave * 32 * DP);
+            else
+                ds = v.dot(do_now + g * 32 * DP);
+            settle<T>(s, ds);
             score.apply<T>(s);
-            f32x16 p = s, ds;            // log2(e) w, then p; the uniform cases stand outside of the loops over elements
-            if (a.slopes) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    p[e] = fmaf(-slope, fabsf(static_cast<float>(pos_tile[in][32 * g + reg_row(e, half)] - j)), p[e]);
-            }
+            // s becomes p, dp becomes ds, in place; what is the same for the whole wave stands outside of the loops over elements
+            const int rows0 = 64 * g + 4 * half;                       // and 8 x further: four rows
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const f32x4 stats = *reinterpret_cast<const f32x4*>(stat_tile[in] + 32 * g + 8 * x + 4 * half);       // of four rows
-                const f32x4 deltas = *reinterpret_cast<const f32x4*>(delta_tile[in] + 32 * g + 8 * x + 4 * half);
+                const f32x4 deltas = *reinterpret_cast<const f32x4*>(stats_now + rows0 + 32 + 8 * x);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[4 * x + e] = exp2_(fmaf(p[4 * x + e], score.mul, stats[e]));
-                    ds[4 * x + e] = p[4 * x + e] * (dp[4 * x + e] - deltas[e]);
-                }
+                for (int e = 0; e < 4; ++e) ds[4 * x + e] -= deltas[e];
             }
             if (score.capped) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) ds[e] *= score.slope(s[e]);
             }
+            if (a.slopes) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[e] = fmaf(-slope, fabsf(static_cast<float>(pos_now[64 * g + reg_row(e, half)] - j)), s[e]);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const f32x4 stats = *reinterpret_cast<const f32x4*>(stats_now + rows0 + 8 * x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * x + e] = exp2_(fmaf(s[4 * x + e], score.mul, stats[e]));
+                    ds[4 * x + e] *= s[4 * x + e];
+                }
+            }
             if (!whole) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int at = 32 * g + reg_row(e, half);
-                    if (j < lo_tile[in][at] || j >= hi_tile[in][at]) p[e] = ds[e] = 0.f;
+                    const int at = 64 * g + reg_row(e, half);
+                    if (j < spans_now[at] || j >= spans_now[at + 32]) s[e] = ds[e] = 0.f;
                 }
             }
             if constexpr (kGain) ds *= gain * kUnshift;
-            Ops<T>::template spread<DP>(dv, do_now + g * 32 * DP, Ops<T>::pack(p));
-            Ops<T>::template spread<DP>(dk, q_now + g * 32 * DP, Ops<T>::pack(ds));
+            Ops<T>::template spread<DP, kFresh>(dv, do_now + g * 32 * DP, Ops<T>::pack(s));
+            if (kFresh) __builtin_amdgcn_sched_barrier(0);
+            Ops<T>::template spread<DP, kFresh>(dk, q_now + g * 32 * DP, Ops<T>::pack(ds));
         }
-        if (more) write_rows(in ^ 1);
     };
     while (more) {                       // both buffers written out, as in the forward kernel
-        step(0, q_even, do_even, q_odd, do_odd);
-        if (more) step(1, q_odd, do_odd, q_even, do_even);
+        step(q_even, do_even, stats_even, spans_even, pos_even, q_odd, do_odd, stats_odd, spans_odd, pos_odd);
+        if (more) step(q_odd, do_odd, stats_odd, spans_odd, pos_odd, q_even, do_even, stats_even, spans_even, pos_even);
     }
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) settle<T>(dk[db], dv[db]);
     if (!real) return;
     write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, kGain ? inverse_gain(gain) * a.scale : a.scale, a.dim);
     write_row<T, DP>(static_cast<T*>(a.dv) + b * a.sdv.batch + j * a.sdv.row + kv * a.sdv.head, dv, kUnshift, a.dim);
@@ -394,19 +408,29 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const D
 
 int groups_of(int nq) { return (nq + kRows - 1) / kRows * 4; }
 
-int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+// Places the parts of Work in a workspace, and returns its size.
+int64_t place(const ddpm_span_attention_args& a, void* workspace, Work* w) {
+    w->groups = groups_of(a.nq);
+    const int64_t rows = static_cast<int64_t>(a.batch) * w->groups, heads = rows * a.heads;
+    char* at = static_cast<char*>(workspace);
+    w->stats = reinterpret_cast<float*>(at);
+    at += heads * 256;
+    w->spans = reinterpret_cast<int*>(at);
+    at += rows * 256;
+    w->positions = reinterpret_cast<int*>(at);
+    at += rows * 256;
+    w->seen = reinterpret_cast<Seen*>(at);
+    at += rows * sizeof(Seen);
+    w->largest = reinterpret_cast<float*>(at);
+    if (a.type == DDPM_F16) at += (heads * 4 + 15) / 16 * 16;
+    return at - static_cast<char*>(workspace);
+}
 
 template <typename T>
 void launch(const ddpm_span_attention_args& a, void* workspace, hipStream_t stream) {
     const Dev d = dev_args(a);
-    Work work = {};
-    work.groups = groups_of(a.nq);
-    char* at = static_cast<char*>(workspace);
-    work.seen = reinterpret_cast<Seen*>(at);
-    at += static_cast<int64_t>(a.batch) * work.groups * sizeof(Seen);
-    work.delta = reinterpret_cast<float*>(at);
-    at += round16(static_cast<int64_t>(a.batch) * a.heads * a.nq * 4);
-    work.largest = reinterpret_cast<float*>(at);
+    Work work;
+    place(a, workspace, &work);
     for_dim(a.dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
         if (a.nq > 0) dq_kernel<T, DP><<<dim3(work.groups / 4, a.heads, a.batch), kThreads, 0, stream>>>(d, work);
@@ -426,10 +450,8 @@ bool check_bwd(const ddpm_span_attention_args& a) {
 
 extern "C" int64_t ddpm_span_attention_bwd_workspace(const ddpm_span_attention_args* a) {
     if (!a || !check_bwd(*a)) return ddpm::fail_invalid("span attention sizes, type or strides");
-    const int64_t groups = groups_of(a->nq);
-    return static_cast<int64_t>(a->batch) * groups * static_cast<int64_t>(sizeof(Seen)) +
-           round16(static_cast<int64_t>(a->batch) * a->heads * a->nq * 4) +
-           (a->type == DDPM_F16 ? round16(static_cast<int64_t>(a->batch) * a->heads * groups * 4) : 0);
+    Work work;
+    return place(*a, nullptr, &work);
 }
 
 extern "C" int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* workspace, void* stream) {

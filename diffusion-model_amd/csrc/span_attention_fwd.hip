@@ -160,10 +160,13 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         if (j0 + kTile <= wlo || j0 >= whi) return;                 // nothing here for this wave's rows
         f32x16 s[kBlocks];
 #pragma unroll
-        for (int kb = 0; kb < kBlocks; ++kb) {
-            s[kb] = q.dot(k_now + kb * 32 * DP);
-            score.apply<T>(s[kb]);
-        }
+        for (int kb = 0; kb < kBlocks; ++kb) s[kb] = q.dot(k_now + kb * 32 * DP);
+        if constexpr (kBlocks == 2)
+            settle<T>(s[0], s[1]);
+        else
+            settle<T>(s[0]);
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; ++kb) score.apply<T>(s[kb]);
         if (a.slopes) {
 #pragma unroll
             for (int kb = 0; kb < kBlocks; ++kb)
@@ -212,6 +215,8 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         if (t + 1 < last) step(t + 1, k_odd, v_odd, k_even, v_even);
     }
 
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) settle<T>(acc[db]);
     sum += other_half(sum);
     if (!real) return;
     const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
