@@ -351,28 +351,25 @@ struct Score {
             s *= pre;
             return;
         }
-        // tanh x = x (1 + x^2 (...)) where all of the wave's scores are small beside the cap, as most are: fitted for the smallest largest
-        // relative error, 6.4e-7 below 0.5 (less than a thousandth of a 16-bit weight's rounding), 3.3e-8 below 0.75 for fp32. It costs
-        // 7 operations for the 11 (an exponential and a reciprocal take four each) of 1 - 2 / (e^2x + 1).
+        // cap tanh x = cap x (1 + x^2 (...)) where all of the wave's scores are small beside the cap, as most are: fitted for the smallest
+        // largest relative error, 6.4e-7 below x = 0.5 (less than a thousandth of a 16-bit weight's rounding), 3.3e-8 below 0.75 for
+        // fp32. With the constants multiplied out for s itself it costs 5 operations (fp32: 7) for the 11 (an exponential and a
+        // reciprocal take four each) of 1 - 2 / (e^2x + 1).
         constexpr bool exact = __is_same(T, float);
         float most = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[r]));
         if (__all(most * pre < (exact ? 0.75f : 0.5f))) {
+            const float c0 = cap * pre, y = pre * pre, c1 = (exact ? -3.333306838e-01f : -3.332815933e-01f) * c0 * y;
+            const float c2 = (exact ? 1.332652116e-01f : 1.320535960e-01f) * c0 * y * y;
+            const float c3 = (exact ? -5.339025798e-02f : -4.475064100e-02f) * c0 * y * y * y;
+            const float c4 = 1.966491225e-02f * c0 * y * y * y * y, c5 = -4.769489293e-03f * c0 * y * y * y * y * y;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float x = s[r] * pre, y = x * x;
-                float p;
-                if constexpr (exact) {
-                    p = fmaf(y, -4.769489293e-03f, 1.966491225e-02f);
-                    p = fmaf(y, p, -5.339025798e-02f);
-                    p = fmaf(y, p, 1.332652116e-01f);
-                    p = fmaf(y, p, -3.333306838e-01f);
-                } else {
-                    p = fmaf(y, -4.475064100e-02f, 1.320535960e-01f);
-                    p = fmaf(y, p, -3.332815933e-01f);
-                }
-                s[r] = x * cap * fmaf(y, p, 1.f);
+                const float z = s[r] * s[r];
+                float p = exact ? fmaf(z, fmaf(z, c5, c4), c3) : c3;
+                p = fmaf(z, fmaf(z, fmaf(z, p, c2), c1), c0);
+                s[r] *= p;
             }
             return;
         }
@@ -407,6 +404,23 @@ __device__ __forceinline__ void write_out(const Dev& a, int64_t at, const float 
     }
     *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at) = high;
     if (sizeof(T) == 2 && a.out_low) *reinterpret_cast<T4*>(static_cast<T*>(a.out_low) + at) = low;
+}
+
+// The block of rows (or keys) x, of gridDim.x, and the pair of head and batch entry that a workgroup takes. Workgroups start in the order
+// of their index and go to the 8 XCDs in turn. Where the pairs are a multiple of 8, pairs run fastest: an XCD, with its L2, keeps to
+// an eighth of the pairs, and all of them start with their first blocks, which the caller makes the longest ones, so that short ones fill
+// up the end. Otherwise neighbouring blocks of one pair go to one XCD.
+struct Place {
+    int x, head, batch;
+};
+__device__ __forceinline__ Place place_of() {
+    const unsigned pairs = gridDim.y * gridDim.z;
+    if (pairs % 8 == 0) {
+        const unsigned id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), pair = id % pairs;
+        return {static_cast<int>(id / pairs), static_cast<int>(pair % gridDim.y), static_cast<int>(pair / gridDim.y)};
+    }
+    const dim3 id = ddpm::xcd_block();
+    return {static_cast<int>(id.x), static_cast<int>(id.y), static_cast<int>(id.z)};
 }
 
 // tile row of register r of this lane half

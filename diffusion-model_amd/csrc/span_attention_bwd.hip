@@ -27,7 +27,8 @@ struct Work {
     int* positions;                      // [batch][groups][32, and 32 unused]
     float* stats;                        // [batch][heads][groups][-lse in units of log 2 plus kShift | D]
     float* largest;                      // fp16: largest |ds| of a group: [batch][heads][groups]
-    int groups;
+    float* sums;                         // split dk/dv kernel: [parts][dk | dv][batch][nk][kv_heads][dim]
+    int groups, parts;
 };
 
 // fp16 has five bits of exponent, and score gradients are as small as a loss makes them: they are scaled by a power of two
@@ -67,8 +68,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     __shared__ __attribute__((aligned(1024))) T k_even[kTile * DP], k_odd[kTile * DP], v_even[kTile * DP], v_odd[kTile * DP];
     __shared__ int bounds[2][4];
 
-    const dim3 id = ddpm::xcd_block();
-    const int block = gridDim.x - 1 - id.x, head = id.y, b = id.z;
+    const Place id = place_of();
+    const int block = gridDim.x - 1 - id.x, head = id.head, b = id.batch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int i = block * kRows + wave * 32 + (lane & 31);
     const bool real = i < a.nq;
@@ -197,11 +198,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
 
 // The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other. What a tile sees comes through
 // scalar loads: a vector load behind the fetches of a tile could only arrive after them.
+// Of `parts` parts (a power of two) that share the tiles of these keys, part p takes those whose number plus the head's leaves p.
 template <int GROUPS>                    // groups of 32 rows in a tile
 struct Tiles {
     typedef const __attribute__((address_space(4))) Seen* Scalar;
     const Seen* seen;
-    int groups, tiles, heads, begin, end;
+    int groups, tiles, heads, begin, end, part, parts;
     int base;                            // 64 tiles from `base` on are in `mask`
     unsigned long long mask;
     // the current one
@@ -214,7 +216,7 @@ struct Tiles {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
             if (t * GROUPS + g < groups) any |= seen[t * GROUPS + g].lo < end && seen[t * GROUPS + g].hi > begin;
-        mask = __ballot(any);
+        mask = __ballot(any && ((t + head) & (parts - 1)) == part);
     }
     __device__ __forceinline__ void start() {
         base = head = 0;
@@ -241,12 +243,14 @@ struct Tiles {
     }
 };
 
-template <typename T, int DP>
+// dk and dv. A workgroup of 4 waves takes 128 keys, 32 a wave, and walks over the rows that see any of them, for every query head
+// that shares them. For 16-bit types of more than 64 channels v stays in LDS and is read for each product, which leaves a wave
+// room beside another on its SIMD (256 registers); with k and v both in registers it would have some 390 and the SIMD for itself, and
+// the matrix unit would wait while it works on scores: 623 TFLOP/s at 128 channels, 828 so. Where there are few keys and many rows
+// the rows are dealt out to several workgroups (SPLIT), whose sums a last kernel adds up.
+template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void dkv_kernel(const Dev a, const Work work) {
-#ifndef VL
-#define VL 64
-#endif
-    constexpr bool kLdsV = sizeof(T) == 2 && DP > VL, kFresh = kLdsV && DP > 96;
+    constexpr bool kLdsV = sizeof(T) == 2 && DP > 64, kFresh = kLdsV && DP > 96;
     constexpr int kTile = kLdsV ? 32 : Ops<T>::kTile, kBlocks = kTile / 32;
     __shared__ __attribute__((aligned(1024))) T v_rows[kLdsV ? kRows * DP : 1];
     constexpr bool kGain = __is_same(T, _Float16);
@@ -256,10 +260,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
     __shared__ __attribute__((aligned(256))) int spans_even[64 * kBlocks], spans_odd[64 * kBlocks], pos_even[64 * kBlocks], pos_odd[64 * kBlocks];
     __shared__ float wave_max[4];
 
-    const dim3 id = ddpm::xcd_block();
-    const int kv = id.y, b = id.z;
+    const Place id = place_of();
+    const int kv = id.head, b = id.batch;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int begin = id.x * kRows, w0 = begin + wave * 32, j = w0 + (lane & 31);   // keys of the workgroup, the wave, the lane
+    const int part = SPLIT ? id.x & (work.parts - 1) : 0;
+    const int begin = (SPLIT ? id.x / work.parts : id.x) * kRows, w0 = begin + wave * 32, j = w0 + (lane & 31);   // keys of the workgroup, the wave, the lane
     const bool real = j < a.nk;
     OwnRow<T, DP> k, v;
     k.load(real ? static_cast<const T*>(a.k) + b * a.sk.batch + j * a.sk.row + kv * a.sk.head : nullptr, a.dim);
@@ -293,6 +298,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
     tiles.heads = a.group;
     tiles.begin = begin;
     tiles.end = min(begin + kRows, a.nk);
+    tiles.part = part;
+    tiles.parts = SPLIT ? work.parts : 1;
     tiles.start();
 
     Fetch<T, DP, kTile> qs, dos;
@@ -402,8 +409,50 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) settle<T>(dk[db], dv[db]);
     if (!real) return;
-    write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, kGain ? inverse_gain(gain) * a.scale : a.scale, a.dim);
-    write_row<T, DP>(static_cast<T*>(a.dv) + b * a.sdv.batch + j * a.sdv.row + kv * a.sdv.head, dv, kUnshift, a.dim);
+    const float fk = kGain ? inverse_gain(gain) * a.scale : a.scale;
+    if (SPLIT) {
+        const int64_t keys = static_cast<int64_t>(gridDim.z) * a.nk * gridDim.y, at = (static_cast<int64_t>(b) * a.nk + j) * gridDim.y + kv;
+        write_row<float, DP>(work.sums + (2 * part * keys + at) * a.dim, dk, fk, a.dim);
+        write_row<float, DP>(work.sums + ((2 * part + 1) * keys + at) * a.dim, dv, kUnshift, a.dim);
+    } else {
+        write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, fk, a.dim);
+        write_row<T, DP>(static_cast<T*>(a.dv) + b * a.sdv.batch + j * a.sdv.row + kv * a.sdv.head, dv, kUnshift, a.dim);
+    }
+}
+
+// Adds up the parts of dk (y = 0) and dv (y = 1), four channels a thread, in the parts' order.
+template <typename T>
+__global__ __launch_bounds__(256) void add_parts_kernel(const Dev a, const Work work, const int kv_heads, const int64_t keys) {
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int quads = a.dim / 4;
+    const int64_t key = id / quads;
+    if (key >= keys) return;
+    const int c = 4 * static_cast<int>(id - key * quads);
+    f32x4 sum = {};
+    for (int p = 0; p < work.parts; ++p) sum += *reinterpret_cast<const f32x4*>(work.sums + ((2 * p + blockIdx.y) * keys + key) * a.dim + c);
+    const int kv = static_cast<int>(key % kv_heads);
+    const int64_t bj = key / kv_heads, b = bj / a.nk, j = bj % a.nk;
+    const Strides& s = blockIdx.y ? a.sdv : a.sdk;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(sum[e]);
+    *reinterpret_cast<T4*>(static_cast<T*>(blockIdx.y ? a.dv : a.dk) + b * s.batch + j * s.row + kv * s.head + c) = o;
+}
+
+// Workgroups that share the rows of a block of keys: as many as bring the call to two workgroups a compute unit, up to 8, with 8
+// tiles each at least. Packed images of 8192 tokens with 4 key/value heads are 256 blocks, one a compute unit, the slowest of which
+// decides: MEASURED.
+#ifndef TB
+#define TB 512
+#define TS 1024
+#endif
+int parts_of(const ddpm_span_attention_args& a) {
+    const int64_t blocks = (static_cast<int64_t>(a.nk) + kRows - 1) / kRows * a.kv_heads * a.batch;
+    const int64_t tiles = (static_cast<int64_t>(a.nq) + 31) / 32 * (a.heads / a.kv_heads);
+    int parts = 1;
+    while (parts < 8 && blocks * parts < (a.spans ? TS : TB) && tiles / (2 * parts) >= 8) parts *= 2;
+    return parts;
 }
 
 int groups_of(int nq) { return (nq + kRows - 1) / kRows * 4; }
@@ -423,6 +472,9 @@ int64_t place(const ddpm_span_attention_args& a, void* workspace, Work* w) {
     at += rows * sizeof(Seen);
     w->largest = reinterpret_cast<float*>(at);
     if (a.type == DDPM_F16) at += (heads * 4 + 15) / 16 * 16;
+    w->sums = reinterpret_cast<float*>(at);
+    w->parts = parts_of(a);
+    if (w->parts > 1) at += static_cast<int64_t>(w->parts) * 2 * a.batch * a.nk * a.kv_heads * a.dim * 4;
     return at - static_cast<char*>(workspace);
 }
 
@@ -434,8 +486,14 @@ void launch(const ddpm_span_attention_args& a, void* workspace, hipStream_t stre
     for_dim(a.dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
         if (a.nq > 0) dq_kernel<T, DP><<<dim3(work.groups / 4, a.heads, a.batch), kThreads, 0, stream>>>(d, work);
-        if (a.nk > 0) dkv_kernel<T, DP><<<dim3((a.nk + kRows - 1) / kRows, a.kv_heads, a.batch), kThreads, 0, stream>>>(d, work);
+        const dim3 grid((a.nk + kRows - 1) / kRows * work.parts, a.kv_heads, a.batch);
+        if (a.nk > 0 && work.parts == 1) dkv_kernel<T, DP, false><<<grid, kThreads, 0, stream>>>(d, work);
+        if (a.nk > 0 && work.parts > 1) dkv_kernel<T, DP, true><<<grid, kThreads, 0, stream>>>(d, work);
     });
+    if (a.nk > 0 && work.parts > 1) {
+        const int64_t keys = static_cast<int64_t>(a.batch) * a.nk * a.kv_heads;
+        add_parts_kernel<T><<<dim3(static_cast<unsigned>((keys * (a.dim / 4) + 255) / 256), 2), 256, 0, stream>>>(d, work, a.kv_heads, keys);
+    }
 }
 
 bool check_bwd(const ddpm_span_attention_args& a) {
@@ -462,7 +520,7 @@ extern "C" int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* 
     for (const void* p : {a->q, a->k, a->v, static_cast<const void*>(a->out), static_cast<const void*>(a->out_low), a->dout, static_cast<const void*>(a->dq),
                           static_cast<const void*>(a->dk), static_cast<const void*>(a->dv), static_cast<const void*>(workspace)})
         DDPM_REQUIRE(ddpm::aligned16(p));
-    DDPM_REQUIRE(a->nq == 0 || workspace);
+    DDPM_REQUIRE(a->nq == 0 || workspace);                // dk and dv of no rows are noughts, and need none
     if (a->type == DDPM_F32)
         launch<float>(*a, workspace, as_stream(stream));
     else if (a->type == DDPM_BF16)

@@ -106,16 +106,16 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
     __shared__ int bounds[2][4];
 
     // x: row blocks (the last first: under causal order they have most to do), and with SPLIT the parts of the keys beside them
-    const dim3 id = ddpm::xcd_block();
+    const Place id = place_of();
     const int part = SPLIT ? id.x % parts.splits : 0;
     const int block = SPLIT ? id.x / parts.splits : gridDim.x - 1 - id.x;
-    const int b = id.z;
+    const int b = id.batch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int r = block * kRows + wave * 32 + (lane & 31);          // row of this lane's column
     const bool real = r < a.nq * pack;
     const int i = real ? r / pack : 0;
-    const int head = id.y * pack + (real ? r % pack : 0);
-    const int kv = (id.y * pack) / a.group;
+    const int head = id.head * pack + (real ? r % pack : 0);
+    const int kv = (id.head * pack) / a.group;
 
     const Row row = real ? row_of(a, b, i) : no_row();
     int wlo = row.lo, whi = row.hi;
