@@ -26,9 +26,10 @@ struct Work {
     int* spans;                          // [batch][groups][lo of 32 rows | hi]
     int* positions;                      // [batch][groups][32, and 32 unused]
     float* stats;                        // [batch][heads][groups][-lse in units of log 2 plus kShift | D]
-    float* largest;                      // fp16: largest |ds| of a group: [batch][heads][groups]
-    float* sums;                         // split dk/dv kernel: [parts][dk | dv][batch][nk][kv_heads][dim]
-    int groups, parts;
+    float* largest;                      // fp16: largest |ds| of a group: [batch][heads][q_parts][groups]
+    float* q_sums;                       // split dq kernel: [q_parts][batch][nq][heads][dim]
+    float* sums;                         // split dk/dv kernel: [dk | dv][parts][batch][nk][kv_heads][dim]
+    int groups, q_parts, parts;
 };
 
 // fp16 has five bits of exponent, and score gradients are as small as a loss makes them: they are scaled by a power of two
@@ -61,7 +62,10 @@ __device__ __forceinline__ void write_row(T* out, const f32x16* acc, float f, in
         }
 }
 
-template <typename T, int DP>
+// dq. A workgroup of 4 waves takes 128 rows of one head, 32 a wave, and walks over the keys that any of them sees; where there are few
+// rows and many keys several workgroups take a tile in turn each (SPLIT), and a last kernel adds up their sums. It also leaves what the
+// other kernel has to know of the rows.
+template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_kernel(const Dev a, const Work work) {
     constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
     constexpr bool kGain = __is_same(T, _Float16);
@@ -69,7 +73,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     __shared__ int bounds[2][4];
 
     const Place id = place_of();
-    const int block = gridDim.x - 1 - id.x, head = id.head, b = id.batch;
+    const int parts = SPLIT ? work.q_parts : 1, part = SPLIT ? id.x % parts : 0;
+    const int block = (gridDim.x - 1 - id.x) / parts, head = id.head, b = id.batch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int i = block * kRows + wave * 32 + (lane & 31);
     const bool real = i < a.nq;
@@ -78,7 +83,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     int wlo = row.lo, whi = row.hi;
     join_rows(wlo, whi);
     const int64_t group = static_cast<int64_t>(b) * work.groups + block * 4 + wave;
-    if (head == 0) {
+    if (head == 0 && part == 0) {
         int alo = row.lo, ahi = row.hi;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
@@ -112,11 +117,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
         delta += other_half(delta);
     }
     if (real) stat = stat_of(a.lse[at]);
-    work.stats[64 * ((static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave) + lane] = half ? delta : Ops<T>::kShift - stat;
+    if (part == 0)
+        work.stats[64 * ((static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave) + lane] = half ? delta : Ops<T>::kShift - stat;
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
-    const int first = lo < hi ? lo / kTile : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;
+    const int first = lo < hi ? lo / kTile + part : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;      // every parts-th tile
 
     const Score score(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
@@ -132,9 +138,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
         arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
-        if (t + 1 < last) {
-            ks.load(k_next, j0 + kTile, a.dim);
-            vs.load(v_next, j0 + kTile, a.dim);
+        if (t + parts < last) {
+            ks.load(k_next, j0 + parts * kTile, a.dim);
+            vs.load(v_next, j0 + parts * kTile, a.dim);
         }
         if (j0 + kTile <= wlo || j0 >= whi) return;
         const bool whole = __all(row.lo <= j0 && row.hi >= j0 + kTile);
@@ -181,19 +187,23 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
             Ops<T>::template spread<DP>(acc, k_now + kb * 32 * DP, Ops<T>::pack(ds));
         }
     };
-    for (int t = first; t < last; t += 2) {          // both buffers written out, as in the forward kernel
+    for (int t = first; t < last; t += 2 * parts) {  // both buffers written out, as in the forward kernel
         step(t, k_even, v_even, k_odd, v_odd);
-        if (t + 1 < last) step(t + 1, k_odd, v_odd, k_even, v_even);
+        if (t + parts < last) step(t + parts, k_odd, v_odd, k_even, v_even);
     }
     if constexpr (kGain) {
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
-        if (lane == 0) work.largest[(static_cast<int64_t>(b) * a.heads + head) * work.groups + block * 4 + wave] = largest;
+        if (lane == 0) work.largest[((static_cast<int64_t>(b) * a.heads + head) * parts + part) * work.groups + block * 4 + wave] = largest;
     }
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) settle<T>(acc[db]);
-    if (real)
-        write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, kGain ? inverse_gain(gain) * a.scale : a.scale, a.dim);
+    if (!real) return;
+    const float f = kGain ? inverse_gain(gain) * a.scale : a.scale;
+    if (SPLIT)
+        write_row<float, DP>(work.q_sums + (((static_cast<int64_t>(part) * gridDim.z + b) * a.nq + i) * a.heads + head) * a.dim, acc, f, a.dim);
+    else
+        write_row<T, DP>(static_cast<T*>(a.dq) + b * a.sdq.batch + i * a.sdq.row + head * a.sdq.head, acc, f, a.dim);
 }
 
 // The tiles of kTile rows that see any of the keys [begin, end), for one query head after the other. What a tile sees comes through
@@ -279,9 +289,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
     if (a.scale < 0.f) k.negate();       // used in scores alone
     float gain = 1.f;
     if constexpr (kGain) {
-        const float* largest = work.largest + (static_cast<int64_t>(b) * a.heads + kv * a.group) * work.groups;
+        const int each = work.groups * work.q_parts;                   // of a head
+        const float* largest = work.largest + (static_cast<int64_t>(b) * a.heads + kv * a.group) * each;
         float m = 0.f;
-        for (int64_t x = threadIdx.x; x < static_cast<int64_t>(a.group) * work.groups; x += kThreads) m = fmaxf(m, largest[x]);
+        for (int64_t x = threadIdx.x; x < static_cast<int64_t>(a.group) * each; x += kThreads) m = fmaxf(m, largest[x]);
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
         if (lane == 0) wave_max[wave] = m;
@@ -412,47 +423,59 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
     const float fk = kGain ? inverse_gain(gain) * a.scale : a.scale;
     if (SPLIT) {
         const int64_t keys = static_cast<int64_t>(gridDim.z) * a.nk * gridDim.y, at = (static_cast<int64_t>(b) * a.nk + j) * gridDim.y + kv;
-        write_row<float, DP>(work.sums + (2 * part * keys + at) * a.dim, dk, fk, a.dim);
-        write_row<float, DP>(work.sums + ((2 * part + 1) * keys + at) * a.dim, dv, kUnshift, a.dim);
+        write_row<float, DP>(work.sums + (part * keys + at) * a.dim, dk, fk, a.dim);
+        write_row<float, DP>(work.sums + ((work.parts + part) * keys + at) * a.dim, dv, kUnshift, a.dim);
     } else {
         write_row<T, DP>(static_cast<T*>(a.dk) + b * a.sdk.batch + j * a.sdk.row + kv * a.sdk.head, dk, fk, a.dim);
         write_row<T, DP>(static_cast<T*>(a.dv) + b * a.sdv.batch + j * a.sdv.row + kv * a.sdv.head, dv, kUnshift, a.dim);
     }
 }
 
-// Adds up the parts of dk (y = 0) and dv (y = 1), four channels a thread, in the parts' order.
+// Adds up the parts of a gradient, four channels a thread, in the parts' order: sums [parts][batch][n][heads][dim] -> out.
 template <typename T>
-__global__ __launch_bounds__(256) void add_parts_kernel(const Dev a, const Work work, const int kv_heads, const int64_t keys) {
+__global__ __launch_bounds__(256) void add_parts_kernel(const float* sums, const int parts, const int64_t rows, const int n, const int heads,
+                                                        const int dim, T* out, const Strides s) {
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int quads = a.dim / 4;
-    const int64_t key = id / quads;
-    if (key >= keys) return;
-    const int c = 4 * static_cast<int>(id - key * quads);
+    const int quads = dim / 4;
+    const int64_t row = id / quads;
+    if (row >= rows) return;
+    const int c = 4 * static_cast<int>(id - row * quads);
     f32x4 sum = {};
-    for (int p = 0; p < work.parts; ++p) sum += *reinterpret_cast<const f32x4*>(work.sums + ((2 * p + blockIdx.y) * keys + key) * a.dim + c);
-    const int kv = static_cast<int>(key % kv_heads);
-    const int64_t bj = key / kv_heads, b = bj / a.nk, j = bj % a.nk;
-    const Strides& s = blockIdx.y ? a.sdv : a.sdk;
+    for (int p = 0; p < parts; ++p) sum += *reinterpret_cast<const f32x4*>(sums + (p * rows + row) * dim + c);
+    const int head = static_cast<int>(row % heads);
+    const int64_t bn = row / heads, b = bn / n, i = bn % n;
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(sum[e]);
-    *reinterpret_cast<T4*>(static_cast<T*>(blockIdx.y ? a.dv : a.dk) + b * s.batch + j * s.row + kv * s.head + c) = o;
+    *reinterpret_cast<T4*>(out + b * s.batch + i * s.row + head * s.head + c) = o;
 }
 
-// Workgroups that share the rows of a block of keys: as many as bring the call to two workgroups a compute unit, up to 8, with 8
-// tiles each at least. Packed images of 8192 tokens with 4 key/value heads are 256 blocks, one a compute unit, the slowest of which
-// decides: MEASURED.
-#ifndef TB
-#define TB 512
-#define TS 1024
-#endif
+template <typename T>
+void add_parts(const float* sums, int parts, int64_t batch, int n, int heads, int dim, void* out, const Strides& s, hipStream_t stream) {
+    const int64_t rows = batch * n * heads;
+    add_parts_kernel<T><<<static_cast<unsigned>((rows * (dim / 4) + 255) / 256), 256, 0, stream>>>(sums, parts, rows, n, heads, dim,
+                                                                                                 static_cast<T*>(out), s);
+}
+
+// Workgroups that share the tiles of a block of rows or keys: a power of two up to 8 that brings the call to `wanted` workgroups, with
+// `least` tiles each at least.
+int parts_for(int64_t blocks, int64_t wanted, int64_t tiles, int least) {
+    int parts = 1;
+    while (parts < 8 && blocks * parts < wanted && tiles / (2 * parts) >= least) parts *= 2;
+    return parts;
+}
+
+// Two workgroups a compute unit fill the chip; spans load them unevenly, and then four are better. dk and dv of 8192 packed tokens in
+// documents of 340, 4 key/value heads shared by 16, are 256 blocks: 1056 us with a workgroup each, 542 with two, 304 with four,
+// 285 with eight; where all rows see all keys 1692 us with one, 1178 with two, 1192 with four.
 int parts_of(const ddpm_span_attention_args& a) {
     const int64_t blocks = (static_cast<int64_t>(a.nk) + kRows - 1) / kRows * a.kv_heads * a.batch;
-    const int64_t tiles = (static_cast<int64_t>(a.nq) + 31) / 32 * (a.heads / a.kv_heads);
-    int parts = 1;
-    while (parts < 8 && blocks * parts < (a.spans ? TS : TB) && tiles / (2 * parts) >= 8) parts *= 2;
-    return parts;
+    return parts_for(blocks, a.spans ? 1024 : 512, (static_cast<int64_t>(a.nq) + 31) / 32 * (a.heads / a.kv_heads), 8);
+}
+int q_parts_of(const ddpm_span_attention_args& a) {
+    const int64_t blocks = (static_cast<int64_t>(a.nq) + kRows - 1) / kRows * a.heads * a.batch;
+    return parts_for(blocks, 512, (static_cast<int64_t>(a.nk) + 63) / 64, 4);
 }
 
 int groups_of(int nq) { return (nq + kRows - 1) / kRows * 4; }
@@ -471,7 +494,10 @@ int64_t place(const ddpm_span_attention_args& a, void* workspace, Work* w) {
     w->seen = reinterpret_cast<Seen*>(at);
     at += rows * sizeof(Seen);
     w->largest = reinterpret_cast<float*>(at);
-    if (a.type == DDPM_F16) at += (heads * 4 + 15) / 16 * 16;
+    w->q_parts = q_parts_of(a);
+    if (a.type == DDPM_F16) at += (heads * w->q_parts * 4 + 15) / 16 * 16;
+    w->q_sums = reinterpret_cast<float*>(at);
+    if (w->q_parts > 1) at += static_cast<int64_t>(w->q_parts) * a.batch * a.nq * a.heads * a.dim * 4;
     w->sums = reinterpret_cast<float*>(at);
     w->parts = parts_of(a);
     if (w->parts > 1) at += static_cast<int64_t>(w->parts) * 2 * a.batch * a.nk * a.kv_heads * a.dim * 4;
@@ -485,14 +511,17 @@ void launch(const ddpm_span_attention_args& a, void* workspace, hipStream_t stre
     place(a, workspace, &work);
     for_dim(a.dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        if (a.nq > 0) dq_kernel<T, DP><<<dim3(work.groups / 4, a.heads, a.batch), kThreads, 0, stream>>>(d, work);
-        const dim3 grid((a.nk + kRows - 1) / kRows * work.parts, a.kv_heads, a.batch);
-        if (a.nk > 0 && work.parts == 1) dkv_kernel<T, DP, false><<<grid, kThreads, 0, stream>>>(d, work);
-        if (a.nk > 0 && work.parts > 1) dkv_kernel<T, DP, true><<<grid, kThreads, 0, stream>>>(d, work);
+        const dim3 rows(work.groups / 4 * work.q_parts, a.heads, a.batch), keys((a.nk + kRows - 1) / kRows * work.parts, a.kv_heads, a.batch);
+        if (a.nq > 0 && work.q_parts == 1) dq_kernel<T, DP, false><<<rows, kThreads, 0, stream>>>(d, work);
+        if (a.nq > 0 && work.q_parts > 1) dq_kernel<T, DP, true><<<rows, kThreads, 0, stream>>>(d, work);
+        if (a.nk > 0 && work.parts == 1) dkv_kernel<T, DP, false><<<keys, kThreads, 0, stream>>>(d, work);
+        if (a.nk > 0 && work.parts > 1) dkv_kernel<T, DP, true><<<keys, kThreads, 0, stream>>>(d, work);
     });
+    if (a.nq > 0 && work.q_parts > 1) add_parts<T>(work.q_sums, work.q_parts, a.batch, a.nq, a.heads, a.dim, a.dq, d.sdq, stream);
     if (a.nk > 0 && work.parts > 1) {
-        const int64_t keys = static_cast<int64_t>(a.batch) * a.nk * a.kv_heads;
-        add_parts_kernel<T><<<dim3(static_cast<unsigned>((keys * (a.dim / 4) + 255) / 256), 2), 256, 0, stream>>>(d, work, a.kv_heads, keys);
+        add_parts<T>(work.sums, work.parts, a.batch, a.nk, a.kv_heads, a.dim, a.dk, d.sdk, stream);
+        add_parts<T>(work.sums + static_cast<int64_t>(work.parts) * a.batch * a.nk * a.kv_heads * a.dim, work.parts, a.batch, a.nk, a.kv_heads, a.dim,
+                     a.dv, d.sdv, stream);
     }
 }
 

@@ -77,6 +77,11 @@ def reference(q, k, v, dout=None, scale=None, softcap=0.0, slopes=None, spans=No
     e_dp = dim * U * (do.abs() @ vd.abs().transpose(2, 3).contiguous())
     ds = scale * p * (dp - delta) * dg
     e_ds = (rho + h + 8 * U) * ds.abs() + abs(scale) * p * ((e_dp + e_delta) * dg + (dp - delta).abs() * eg)
+    # An exponential or a product below 2^-126, the smallest normal float, is nought: p may lack all of so small a weight, ds that times
+    # its other factors and, as a product, another 2^-126; each of the n terms of a sum may lack as much.
+    tiny = torch.where(see, 2.0 ** -126, 0.0)
+    e_p = (rho + h) * p + tiny
+    e_ds = e_ds + tiny * (1 + abs(scale) * (dp - delta).abs() * dg)
     if half:
         e_ds = torch.where(see, e_ds + 2.0 ** -36 * ds.abs().amax((2, 3), keepdim=True), 0.0)
     share = lambda x: x.reshape(b, kvh, g, nk, dim).sum(2).transpose(1, 2)              # noqa: E731
@@ -86,7 +91,9 @@ def reference(q, k, v, dout=None, scale=None, softcap=0.0, slopes=None, spans=No
     dk, dv = share(dst @ qd), share(pt @ do)
     n = nq * g * U
     got["dk"] = dk, share(e_ds.transpose(2, 3).contiguous() @ qd.abs()) + n * share(dst.abs() @ qd.abs()) + h * dk.abs()
-    got["dv"] = dv, share(((rho + h) * p).transpose(2, 3).contiguous() @ do.abs()) + n * share(pt @ do.abs()) + h * dv.abs()
+    got["dv"] = dv, share(e_p.transpose(2, 3).contiguous() @ do.abs()) + n * share(pt @ do.abs()) + h * dv.abs()
+    for name, terms in (("dq", nk), ("dk", nq * g), ("dv", nq * g)):
+        got[name] = got[name][0], got[name][1] + terms * 2.0 ** -126
     if half:                                                    # the smallest steps of the type
         for name in ("out", "dq", "dk", "dv"):
             got[name] = got[name][0], got[name][1] + 2.0 ** -25

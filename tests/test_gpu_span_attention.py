@@ -127,6 +127,17 @@ def test_few_rows_against_many_keys(dtype, batch, nq, nk, heads, kv, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [(40, 1500, 4, 1, 64), (700, 700, 2, 2, 32), (1100, 600, 3, 1, 128), (2100, 90, 2, 1, 96), (1, 2000, 2, 2, 40)])
+def test_gradients_whose_work_is_dealt_out(dtype, nq, nk, heads, kv, dim):
+    """Few blocks of rows (or keys) against many of the other: several workgroups share a block, and their sums are added up."""
+    q, k, v, dout = _inputs(1, nq, nk, heads, kv, dim, dtype)
+    g = torch.Generator().manual_seed(0)
+    ends = torch.sort(torch.randint(-50, nk + 50, (1, nq, 2), generator=g), -1).values.int().cuda()
+    _check_all(q, k, v, dout, softcap=15.0, slopes=_slopes(heads))
+    _check_all(q, k, v, dout, spans=ends, causal=nq > nk)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_what_padding_holds_does_not_matter(dtype, bad):
     """NaN and infinities in keys that no row sees and in rows that see no key: outputs and gradients as with noughts there."""
