@@ -3,8 +3,12 @@
 There is deliberately no fallback: if the library is missing or a call fails, an exception is
 raised. Device pointers are passed as integers (tensor.data_ptr()).
 """
+import contextlib
 import ctypes as C
 import os
+import struct
+
+import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DDPM_LIB") or os.path.join(_HERE, "libddpm_mi355x.so")   # DDPM_LIB: diagnostic builds
@@ -50,6 +54,16 @@ class SpanAttentionArgs(C.Structure):
                [(n, I64 * 3) for n in ("dout_stride", "dq_stride", "dk_stride", "dv_stride")]
 
 
+def packer(structure):
+    """`pack` of all fields of a ctypes structure, the elements of an array one after the other, into bytes that stand for it in
+    a call: a few times quicker than setting the fields one by one."""
+    def code(t):
+        return code(t._type_) * t._length_ if hasattr(t, "_length_") else t._type_
+    s = struct.Struct("".join(code(t) for _, t in structure._fields_))
+    assert s.size == C.sizeof(structure)
+    return s.pack
+
+
 _SIGNATURES = {
     "ddpm_abi_version": [],
     "ddpm_schedule_betas": [I32, I32, F64, F64, P],
@@ -65,7 +79,7 @@ _SIGNATURES = {
     "ddpm_mse_fwd": [P, P, I64, P, P, P],
     "ddpm_mse_bwd": [P, P, P, I64, P, P],
     "ddpm_time_embed": [C.POINTER(EmbedArgs), P],
-    "ddpm_rotary": [C.POINTER(RotaryArgs), P],
+    "ddpm_rotary": [P, P],
     "ddpm_sinusoidal_embedding": [P, I32, I32, I32, P, P],
     "ddpm_conv3x3_fwd": [C.POINTER(ConvDesc), P, P, P, C.POINTER(Epilogue), P, P],
     "ddpm_conv1x1_fwd": [C.POINTER(ConvDesc), P, P, P, C.POINTER(Epilogue), P, P],
@@ -103,8 +117,8 @@ _SIGNATURES = {
     "ddpm_attention_bwd": [P, P, I32, P, P, P, P, P, P, P, I32, I32, I32, I32, P],
     "ddpm_attention_fwd": [P, P, I32, P, P, I32, P, P, P, I32, I32, I32, I32, P],
     "ddpm_self_attention_infer": [P, I32, P, P, P, P, P, I32, P, I32, I32, I32, I32, P],
-    "ddpm_span_attention_fwd": [C.POINTER(SpanAttentionArgs), P, P],
-    "ddpm_span_attention_bwd": [C.POINTER(SpanAttentionArgs), P, P],
+    "ddpm_span_attention_fwd": [P, P, P],
+    "ddpm_span_attention_bwd": [P, P, P],
     "ddpm_softmax_rows": [P, I64, I32, P, P],
     "ddpm_inception_split_scores": [P, I64, I32, I32, P, P],
     "ddpm_mean_cov": [P, I64, I32, P, P, P, P],
@@ -149,7 +163,7 @@ def lib():
         handle.ddpm_grad_norm_workspace_doubles.argtypes = [I32]
         for name in ("ddpm_span_attention_fwd_workspace", "ddpm_span_attention_bwd_workspace"):
             getattr(handle, name).restype = C.c_int64
-            getattr(handle, name).argtypes = [C.POINTER(SpanAttentionArgs)]
+            getattr(handle, name).argtypes = [P]
         for name, sig in _SIGNATURES.items():
             fn = getattr(handle, name)          # AttributeError if the header and library disagree
             fn.argtypes = sig
@@ -208,6 +222,19 @@ class math_scope:
         if self.prev is not None:
             set_conv_math(self.prev)
         return False
+
+
+def stream_of(gpu):
+    """Address of the current stream of a GPU, given by its index."""
+    return torch._C._cuda_getCurrentRawStream(gpu)
+
+
+_ALREADY = contextlib.nullcontext()
+
+
+def on_gpu(gpu):
+    """with on_gpu(index): the GPU is the current one. Nothing to do where it is already, which it mostly is."""
+    return _ALREADY if torch.cuda.current_device() == gpu else torch.cuda.device(gpu)
 
 
 def call(name, *args):

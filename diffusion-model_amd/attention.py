@@ -2,11 +2,9 @@
 distance, and masks in which every row sees one span of keys (documents packed into a sequence, prefixes, padded lengths,
 windows, causal order), with its gradient. It stands beside the UNet's own self-attention (second-iteration/unet.py:39-61: one
 head, every pixel sees every pixel) for networks over tokens of images, video and text."""
-import ctypes as C
-
 import torch
 
-from ._lib import SpanAttentionArgs, call, lib
+from ._lib import SpanAttentionArgs, call, lib, on_gpu, packer, stream_of
 
 _TYPES = {torch.float32: (0, 4), torch.bfloat16: (1, 8), torch.float16: (2, 8)}      # DDPM_* code, elements of 16 bytes
 MAX_DIM = 128
@@ -62,57 +60,51 @@ def key_spans(rows, keys=None, *, documents=None, prefix=None, lengths=None, win
 
 
 def _fit(x, width):
-    """x, or a copy, with neighbouring channels on 16-byte boundaries, and 64 rows within 2 GiB."""
-    if (x.stride(3) != 1 or x.data_ptr() % 16 or any(n > 1 and s % width for n, s in zip(x.shape[:3], x.stride()))
-            or x.shape[1] > 1 and x.stride(1) * x.element_size() >= 1 << 25):
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+    """x, or a copy, with neighbouring channels on 16-byte boundaries and 64 rows within 2 GiB; and its strides."""
+    batch, rows, heads, dim = x.shape
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, (rows * heads * dim, heads * dim, dim)
+    strides = [s if n > 1 else 0 for n, s in zip(x.shape, x.stride())]
+    if (x.stride(3) != 1 or x.data_ptr() % 16 or any(s % width for s in strides[:3])
+            or strides[1] * x.element_size() >= 1 << 25):
+        return x.clone(memory_format=torch.contiguous_format), (rows * heads * dim, heads * dim, dim)
+    return x, strides[:3]
 
 
-def _put(a, name, x, stride):
-    setattr(a, name, x.data_ptr())
-    getattr(a, stride)[:] = [s if n > 1 else 0 for n, s in zip(x.shape[:3], x.stride())]
+def _address(x):
+    return 0 if x is None else x.data_ptr()
 
 
-def _arguments(q, k, v, out, low, lse, how):
+_pack = packer(SpanAttentionArgs)
+_NO_GRADIENT = (0,) * 16
+
+
+def _run(entry, q, k, v, out, low, lse, how, gradient=_NO_GRADIENT):
+    """q, k, v, out: (tensor, strides). Runs on the current GPU, the tensors' own."""
     scale, softcap, slopes, spans, positions, causal = how
-    a = SpanAttentionArgs()
-    a.type = _TYPES[q.dtype][0]
-    a.batch, a.nq, a.heads, a.dim = q.shape
-    a.nk, a.kv_heads = k.shape[1], k.shape[2]
-    a.causal, a.scale, a.softcap = causal, scale, softcap
-    if slopes is not None:
-        a.slopes = slopes.data_ptr()
-    if spans is not None:
-        a.spans, a.span_batch_stride = spans.data_ptr(), spans.stride(0) if spans.shape[0] > 1 else 0
-    if positions is not None:
-        a.positions, a.position_batch_stride = positions.data_ptr(), positions.stride(0) if positions.shape[0] > 1 else 0
-    _put(a, "q", q, "q_stride")
-    _put(a, "k", k, "k_stride")
-    _put(a, "v", v, "v_stride")
-    _put(a, "out", out, "out_stride")
-    if low is not None:
-        a.out_low = low.data_ptr()
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    return a
-
-
-def _run(entry, a, device):
-    size = getattr(lib(), entry + "_workspace")(C.byref(a))
-    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
-    call(entry, C.byref(a), C.c_void_p(workspace.data_ptr() if size > 0 else None), C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    x, y = q[0], k[0]
+    batch, rows, heads, dim = x.shape
+    _, keys, kv_heads, _ = y.shape
+    a = _pack(_TYPES[x.dtype][0], batch, rows, keys, heads, kv_heads, dim, causal, scale, softcap, _address(slopes), _address(spans),
+              _address(positions), spans.stride(0) if spans is not None and spans.shape[0] > 1 else 0,
+              positions.stride(0) if positions is not None and positions.shape[0] > 1 else 0, x.data_ptr(), y.data_ptr(), v[0].data_ptr(),
+              out[0].data_ptr(), _address(low), _address(lse), *q[1], *k[1], *v[1], *out[1], *gradient)
+    size = getattr(lib(), entry + "_workspace")(a)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
+    call(entry, a, _address(workspace), stream_of(x.get_device()))
 
 
 def _forward(q, k, v, how, with_lse, with_low=False):
     width = _TYPES[q.dtype][1]
-    q, k, v = (_fit(x, width) for x in (q, k, v))
-    with torch.cuda.device(q.device):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if with_lse else None
-        low = torch.empty_like(out) if with_low and q.dtype != torch.float32 else None
-        _run("ddpm_span_attention_fwd", _arguments(q, k, v, out, low, lse, how), q.device)
-    return q, k, v, out, low, lse
+    q, k, v = _fit(q, width), _fit(k, width), _fit(v, width)
+    x = q[0]
+    batch, rows, heads, dim = x.shape
+    with on_gpu(x.get_device()):
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        lse = torch.empty((batch, heads, rows), dtype=torch.float32, device=x.device) if with_lse else None
+        low = torch.empty_like(out) if with_low and x.dtype != torch.float32 else None
+        _run("ddpm_span_attention_fwd", q, k, v, _fit(out, width), low, lse, how)
+    return x, k[0], v[0], out, low, lse
 
 
 class _SpanAttention(torch.autograd.Function):
@@ -132,15 +124,14 @@ class _SpanAttention(torch.autograd.Function):
             return (None,) * 9
         q, k, v, out, low, lse, slopes, spans, positions = ctx.saved_tensors
         scale, softcap, causal = ctx.how
-        dout = _fit(dout, _TYPES[q.dtype][1])
-        with torch.cuda.device(q.device):
+        width = _TYPES[q.dtype][1]
+        with on_gpu(q.get_device()):
+            dout, ds = _fit(dout, width)
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-            a = _arguments(q, k, v, out, low, lse, (scale, softcap, slopes, spans, positions, causal))
-            _put(a, "dout", dout, "dout_stride")
-            _put(a, "dq", dq, "dq_stride")
-            _put(a, "dk", dk, "dk_stride")
-            _put(a, "dv", dv, "dv_stride")
-            _run("ddpm_span_attention_bwd", a, q.device)
+            (_, qs), (_, ks) = _fit(dq, width), _fit(dk, width)
+            gradient = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ds, *qs, *ks, *ks
+            _run("ddpm_span_attention_bwd", _fit(q, width), _fit(k, width), _fit(v, width), _fit(out, width), low, lse,
+                 (scale, softcap, slopes, spans, positions, causal), gradient)
         return dq, dk, dv, None, None, None, None, None, None
 
 

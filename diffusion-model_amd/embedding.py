@@ -5,7 +5,7 @@ import ctypes as C
 import torch
 import torch.nn as nn
 
-from ._lib import RotaryArgs, call
+from ._lib import RotaryArgs, call, on_gpu, packer, stream_of
 
 
 class SinusoidalTimeEmbedding(nn.Module):
@@ -39,21 +39,24 @@ def grid_positions(*sizes, device="cuda"):
     return torch.stack(torch.meshgrid(*axes, indexing="ij"), -1).reshape(-1, len(sizes))
 
 
+_pack = packer(RotaryArgs)
+_ptr = torch.Tensor.data_ptr
+
+
 def _turn(tensors, positions, axes, base, interleaved, inverse):
-    a = RotaryArgs()
     tensors = [x if x.stride(3) == 1 else x.contiguous() for x in tensors]
     first = tensors[0]
-    outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors]
-    a.type, a.batch, a.tokens, a.dim = _TYPES[first.dtype], first.shape[0], first.shape[1], first.shape[3]
-    a.axes, a.axis_dim = len(axes), (C.c_int32 * 4)(*axes)
-    a.interleaved, a.inverse, a.base, a.tensors = bool(interleaved), bool(inverse), float(base), len(tensors)
-    a.positions, a.position_type = positions.data_ptr(), _POSITION_TYPES[positions.dtype]
-    a.position_batch_stride = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
-    for i, (x, y) in enumerate(zip(tensors, outs)):
-        a.heads[i], a.x[i], a.out[i] = x.shape[2], x.data_ptr(), y.data_ptr()
-        a.x_stride[i][:], a.out_stride[i][:] = x.stride()[:3], y.stride()[:3]
-    with torch.cuda.device(first.device):
-        call("ddpm_rotary", C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    batch, tokens, _, dim = first.shape
+    gpu = first.get_device()
+    with on_gpu(gpu):
+        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors]
+        spare = 2 - len(tensors)                                # no k
+        strides = [n for s in (tensors, outs) for n in (*(n for x in s for n in x.stride()[:3]), *(0,) * 3 * spare)]
+        heads, *pointers = ((*values, *(0,) * spare) for values in ([x.shape[2] for x in tensors], map(_ptr, tensors), map(_ptr, outs)))
+        a = _pack(_TYPES[first.dtype], batch, tokens, dim, len(axes), *axes, *(0,) * (4 - len(axes)), bool(interleaved), inverse,
+                  _POSITION_TYPES[positions.dtype], len(tensors), *heads, base, _ptr(positions),
+                  positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0, *pointers[0], *pointers[1], *strides)
+        call("ddpm_rotary", a, stream_of(gpu))
     return outs
 
 
@@ -100,5 +103,9 @@ def rotary(q, k, positions, axes, base=10000.0, interleaved=False):
         raise ValueError(f"rotary: positions are [tokens][axes] or [batch][tokens][axes] for {(batch, tokens, len(axes))}, got {tuple(positions.shape)}")
     if not all(x.is_cuda and x.device == q.device for x in (*tensors, positions)):
         raise RuntimeError("rotary runs on the MI355X only: q, k and positions must be on one GPU")
-    out = _Rotary.apply(positions.contiguous(), axes, base, interleaved, *tensors)
+    positions = positions.contiguous()
+    if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+        out = _Rotary.apply(positions, axes, float(base), interleaved, *tensors)
+    else:
+        out = tuple(_turn(tensors, positions, axes, float(base), interleaved, False))
     return out[0] if k is None else out

@@ -15,7 +15,7 @@ from operator import attrgetter
 
 import torch
 
-from ._lib import call, lib
+from ._lib import call, lib, on_gpu, stream_of
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # DDPM_F32, DDPM_BF16, DDPM_F16
 _NORMS = {2.0: 0, math.inf: 1}                                        # DDPM_NORM_2, DDPM_NORM_MAX
@@ -27,10 +27,6 @@ def _array(code, values):
     """(address, owner) of a C array of `values`."""
     a = array(code, values)
     return C.c_void_p(a.buffer_info()[0]), a
-
-
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 def _one_gpu(what, tensors):
@@ -69,11 +65,11 @@ class _Norm:
             _distinct(what, pointers, sizes)
         (self.pointers, a), (self.numel, b), (self.types, c) = _array("Q", pointers), _array("q", sizes), _array("i", types)
         self._owners = (a, b, c)
-        with torch.cuda.device(self.device):
+        with on_gpu(self.device):
             workspace = torch.empty(lib().ddpm_grad_norm_workspace_doubles(self.n), dtype=torch.float64, device="cuda")
             self.state = torch.empty(2, dtype=torch.float32, device="cuda")
             call("ddpm_grad_norm", self.n, self.pointers, self.numel, self.types, _NORMS[norm_type], float(max_norm),
-                 C.c_void_p(workspace.data_ptr()), C.c_void_p(self.state.data_ptr()), _stream(self.device))
+                 C.c_void_p(workspace.data_ptr()), C.c_void_p(self.state.data_ptr()), stream_of(self.device))
 
     def factor(self):
         return C.c_void_p(self.state.data_ptr() + 4)
@@ -108,8 +104,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     norm = _Norm("clip_grad_norm_", dense, max_norm, float(norm_type))
     if error_if_nonfinite and not math.isfinite(norm.state[0].item()):
         raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
-    with torch.cuda.device(norm.device):
-        call("ddpm_clip_grads", norm.n, norm.pointers, norm.numel, norm.types, norm.factor(), _stream(norm.device))
+    with on_gpu(norm.device):
+        call("ddpm_clip_grads", norm.n, norm.pointers, norm.numel, norm.types, norm.factor(), stream_of(norm.device))
         if dense is not grads:
             for g, d in zip(grads, dense):
                 if g is not d:
@@ -123,7 +119,7 @@ def _update(lists, pointers, sizes, step, lr, beta1, beta2, eps, weight_decay, f
     arrays = [_array("Q", x) for x in pointers]
     numel = _array("q", sizes)
     args = (len(sizes), *(a[0] for a in arrays), numel[0], float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), step)
-    stream = _stream(torch.cuda.current_device())
+    stream = stream_of(torch.cuda.current_device())
     if factor is None:
         call("ddpm_adam_step", *args, stream)
     else:
@@ -154,7 +150,7 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         raise RuntimeError("adam_step_ (HIP): gradients and moments must match their parameters in size")
     pointers = [list(map(_ptr, x)) for x in lists]
     _distinct("adam_step_", pointers[0] + pointers[2] + pointers[3], sizes * 3)
-    with torch.cuda.device(gpu):
+    with on_gpu(gpu):
         norm = _Norm("adam_step_", lists[1], max_norm, 2.0, pointers[1], sizes) if max_norm is not None else None
         _update(lists, pointers, sizes, int(step), lr, *betas, eps, weight_decay, norm and norm.factor())
     return norm and norm.state[0]
@@ -215,7 +211,7 @@ class Adam(torch.optim.Optimizer):
             norm = _Norm("Adam", [t[1] for _, _, items in work for t in items], self.max_grad_norm, 2.0)
             self.grad_norm = norm.state[0]
         for group, step, items in work:
-            with torch.cuda.device(items[0][0].device):
+            with on_gpu(items[0][0].get_device()):
                 lists = [list(x) for x in zip(*items)]
                 _update(lists, [list(map(_ptr, x)) for x in lists], list(map(_numel, lists[0])), step, group["lr"], *group["betas"], group["eps"], group["weight_decay"],
                         norm and norm.factor())
