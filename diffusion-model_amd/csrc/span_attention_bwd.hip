@@ -157,17 +157,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
                 for (int e = 0; e < 16; ++e) ds[e] *= score.slope(s[e]);
             }
             if (a.slopes) {
+                const float here = static_cast<float>(row.pos - (j0 + 4 * half));
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[e] = fmaf(-slope, fabsf(static_cast<float>(row.pos - (j0 + 32 * kb + reg_row(e, half)))), s[e]);
+                for (int e = 0; e < 16; ++e) s[e] = fmaf(-slope, fabsf(here - static_cast<float>(32 * kb + reg_row(e, 0))), s[e]);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) ds[e] *= exp2_(fmaf(s[e], score.mul, -stat));
-            if (!whole) {
+            if (!whole) {                // one comparison: a row that sees none has lo = INT_MAX, hi = 0, and both sides wrap
+                const int from = j0 + 4 * half - row.lo;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int j = j0 + 32 * kb + reg_row(e, half);
-                    if (j < row.lo || j >= row.hi) ds[e] = 0.f;
+                    const int c = 32 * kb + reg_row(e, 0);
+                    if (static_cast<unsigned>(from + c) >= static_cast<unsigned>(row.hi - row.lo)) ds[e] = 0.f;
                 }
             }
             if constexpr (kGain) {
