@@ -6,6 +6,7 @@
 // 1e19, and at two elements per clock and compute unit far below the float64 rate), per thread, per workgroup and over
 // the workgroups in a fixed order: the same gradients give the same bits.
 #include <cmath>
+#include <type_traits>
 
 #include "tensor_list.h"
 
@@ -59,23 +60,69 @@ __device__ __forceinline__ double take(double acc, float g) {
     return MAXIMUM ? keep_max(acc, fabs(d)) : fma(d, d, acc);
 }
 
-// elements [begin, end) of one tensor, begin a multiple of kChunk
-template <typename T, bool MAXIMUM>
-__device__ __forceinline__ double norm_chunk(const T* __restrict__ p, int64_t begin, int64_t end, double acc) {
+// The elements of a chunk [p, p + n) on their way through a thread's registers: all of its loads are in flight before the first is
+// used, behind a tensor's end too. A last chunk of 8191 elements taken one by one took longer than the rest of a launch:
+// 26.5 us for the norm of 133 tensors of 62 MB and 26.2 us for their clipping, 17.5 and 21.9 us so.
+template <typename T>
+struct Chunk {
     typedef typename Wide<T>::type V;
-    constexpr int W = 16 / sizeof(T), kLoads = static_cast<int>(kChunk) / (kThreads * W);
-    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && end - begin == kChunk) {
-        V v[kLoads];
+    static constexpr int W = 16 / sizeof(T), kLoads = static_cast<int>(kChunk) / (kThreads * W), kSingle = 8;
+
+    // f(element) -> new value; stored where STORE. Noughts stand for elements behind the end.
+    template <bool STORE, typename F>
+    static __device__ __forceinline__ void each(T* __restrict__ p, int n, F f) {
+        int done = 0;
+        if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+            const int vectors = n / W;
+            V v[kLoads];
+            V* q = reinterpret_cast<V*>(p);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) v[i] = reinterpret_cast<const V*>(p + begin)[i * kThreads + threadIdx.x];
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = i * kThreads + threadIdx.x;
+                v[i] = V{};
+                if (at < vectors) v[i] = q[at];
+            }
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = i * kThreads + threadIdx.x;
 #pragma unroll
-            for (int e = 0; e < W; ++e) acc = take<MAXIMUM>(acc, static_cast<float>(v[i][e]));
-    } else {
-        for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) acc = take<MAXIMUM>(acc, static_cast<float>(p[i]));
+                for (int e = 0; e < W; ++e) v[i][e] = f(v[i][e]);
+                if (STORE && at < vectors) q[at] = v[i];
+            }
+            done = vectors * W;
+        }
+        for (int first = done + threadIdx.x; first < n; first += kSingle * kThreads) {
+            T x[kSingle];
+#pragma unroll
+            for (int i = 0; i < kSingle; ++i) {
+                const int at = first + i * kThreads;
+                x[i] = at < n ? p[at] : static_cast<T>(0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < kSingle; ++i) {
+                const int at = first + i * kThreads;
+                x[i] = f(x[i]);
+                if (STORE && at < n) p[at] = x[i];
+            }
+        }
     }
-    return acc;
+};
+
+// f<T>(first element, elements) of every chunk of this workgroup
+template <typename F>
+__device__ __forceinline__ void each_chunk(const List& l, F f) {
+    const int chunks = l.map.first[l.map.count];
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int t = ddpm::tensor_of_chunk(l.map, c);
+        const int64_t begin = static_cast<int64_t>(c - l.map.first[t]) * kChunk;
+        const int n = static_cast<int>(kChunk < l.n[t] - begin ? kChunk : l.n[t] - begin);
+        if (l.type[t] == DDPM_F32)
+            f(static_cast<float*>(l.p[t]) + begin, n);
+        else if (l.type[t] == DDPM_BF16)
+            f(static_cast<__bf16*>(l.p[t]) + begin, n);
+        else
+            f(static_cast<_Float16*>(l.p[t]) + begin, n);
+    }
 }
 
 // v of every thread of the workgroup, joined in a fixed order; valid in thread 0
@@ -94,18 +141,13 @@ __device__ __forceinline__ double join_block(double v) {
 template <bool MAXIMUM>
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const List l, double* __restrict__ partial) {
     double acc = 0.0;
-    const int chunks = l.map.first[l.map.count];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int t = ddpm::tensor_of_chunk(l.map, c);
-        const int64_t begin = static_cast<int64_t>(c - l.map.first[t]) * kChunk;
-        const int64_t end = begin + kChunk < l.n[t] ? begin + kChunk : l.n[t];
-        if (l.type[t] == DDPM_F32)
-            acc = norm_chunk<float, MAXIMUM>(static_cast<const float*>(l.p[t]), begin, end, acc);
-        else if (l.type[t] == DDPM_BF16)
-            acc = norm_chunk<__bf16, MAXIMUM>(static_cast<const __bf16*>(l.p[t]), begin, end, acc);
-        else
-            acc = norm_chunk<_Float16, MAXIMUM>(static_cast<const _Float16*>(l.p[t]), begin, end, acc);
-    }
+    each_chunk(l, [&](auto* p, int n) __attribute__((always_inline)) {
+        using T = std::remove_reference_t<decltype(*p)>;
+        Chunk<T>::template each<false>(p, n, [&](T g) __attribute__((always_inline)) {
+            acc = take<MAXIMUM>(acc, static_cast<float>(g));
+            return g;
+        });
+    });
     acc = join_block<kThreads, MAXIMUM>(acc);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
@@ -125,41 +167,13 @@ __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void scale_chunk(T* __restrict__ p, int64_t begin, int64_t end, float f) {
-    typedef typename Wide<T>::type V;
-    constexpr int W = 16 / sizeof(T), kLoads = static_cast<int>(kChunk) / (kThreads * W);
-    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && end - begin == kChunk) {
-        V v[kLoads];
-        V* q = reinterpret_cast<V*>(p + begin) + threadIdx.x;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) v[i] = q[i * kThreads];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) v[i][e] = static_cast<T>(static_cast<float>(v[i][e]) * f);
-            q[i * kThreads] = v[i];
-        }
-    } else {
-        for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) p[i] = static_cast<T>(static_cast<float>(p[i]) * f);
-    }
-}
-
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const List l, const float* __restrict__ factor) {
     const float f = factor[0];
     if (f == 1.f) return;      // inside the bound: every product would be the gradient itself
-    const int chunks = l.map.first[l.map.count];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int t = ddpm::tensor_of_chunk(l.map, c);
-        const int64_t begin = static_cast<int64_t>(c - l.map.first[t]) * kChunk;
-        const int64_t end = begin + kChunk < l.n[t] ? begin + kChunk : l.n[t];
-        if (l.type[t] == DDPM_F32)
-            scale_chunk(static_cast<float*>(l.p[t]), begin, end, f);
-        else if (l.type[t] == DDPM_BF16)
-            scale_chunk(static_cast<__bf16*>(l.p[t]), begin, end, f);
-        else
-            scale_chunk(static_cast<_Float16*>(l.p[t]), begin, end, f);
-    }
+    each_chunk(l, [&](auto* p, int n) __attribute__((always_inline)) {
+        using T = std::remove_reference_t<decltype(*p)>;
+        Chunk<T>::template each<true>(p, n, [&](T g) __attribute__((always_inline)) { return static_cast<T>(static_cast<float>(g) * f); });
+    });
 }
 
 bool known_type(int t) { return t == DDPM_F32 || t == DDPM_BF16 || t == DDPM_F16; }
