@@ -80,9 +80,15 @@ def _gradients(what, parameters):
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [g for g in map(_grad, parameters) if g is not None]
+    try:
+        dense = all(map(_contiguous, grads))                    # raises for a sparse one, which spares the others a question
+    except (RuntimeError, NotImplementedError):
+        dense = False
+    if dense:
+        return grads, grads
     if any(g.layout != torch.strided for g in grads):
         raise RuntimeError(f"{what} does not support sparse gradients")
-    return grads, grads if all(map(_contiguous, grads)) else [g.contiguous() for g in grads]
+    return grads, [g.contiguous() for g in grads]
 
 
 @torch.no_grad()

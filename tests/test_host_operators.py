@@ -222,3 +222,18 @@ def test_reference_gradient_against_differences():
         at = [(reference(*(y + s * e if y is x else y for y in (q, k, v)), **how)["out"][0] * dout).sum() for s in (1e-5, -1e-5)]
         assert abs(float((at[0] - at[1]) / 2e-5 - (want[name][0] * e).sum())) < 1e-7
     assert (want["out"][0][:, [2, 4]] == 0).all() and (want["dq"][0][:, [2, 4]] == 0).all()
+
+
+@pytest.mark.parametrize("layout", ["coo", "csr"])
+def test_clip_refuses_sparse_gradients(layout):
+    p = torch.nn.Parameter(torch.zeros(3, 4))
+    q = torch.nn.Parameter(torch.zeros(3))
+    dense = torch.eye(3, 4)
+    q.grad = torch.ones(3)
+    p.grad = dense.to_sparse()
+    if layout == "csr":
+        p = torch.nn.Parameter(torch.zeros(3, 4).to_sparse_csr())
+        p.grad = dense.to_sparse_csr()
+    for f in (lambda: optim.clip_grad_norm_([q, p], 1.0), lambda: optim.grad_norm([q, p])):
+        with pytest.raises(RuntimeError, match="sparse"):
+            f()
