@@ -154,9 +154,16 @@ struct Ops {                             // bf16, fp16
         for (int r = 0; r < 16; ++r) w.f[r >> 3][r & 7] = static_cast<T>(p[r]);
         return w;
     }
-    // acc[db] += over 32 tile rows; `tile` points at the first of them
+    // what pack() left of p
+    static __device__ __forceinline__ Weights rest(const f32x16& p, const Weights& w) {
+        Weights low;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) low.f[r >> 3][r & 7] = static_cast<T>(p[r] - static_cast<float>(w.f[r >> 3][r & 7]));
+        return low;
+    }
+    // acc[db] += over 32 tile rows; `tile` points at the first of them. With `low` the weights are w + low.
     template <int DP, bool FRESH = false>
-    static __device__ __forceinline__ void spread(f32x16* acc, const T* tile, const Weights& w) {
+    static __device__ __forceinline__ void spread(f32x16* acc, const T* tile, const Weights& w, const Weights* low = nullptr) {
         // The transposing read gives lane l of 16 the column l of a 4 x 16 block whose rows four lanes each point at: rows
         // 4 h ... 4 h + 3 (and 8 further) are the ones whose weights this lane half holds.
         const int lane = threadIdx.x & 63, l16 = lane & 15, row = 4 * (lane >> 5) + (l16 >> 2);
@@ -172,6 +179,7 @@ struct Ops {                             // bf16, fp16
             for (int db = 0; db < DP / 32; ++db) {
                 const auto xy = __builtin_shufflevector(four(16 * t, db), four(16 * t + 8, db), 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[db] = mfma(__builtin_bit_cast(Frag, xy), w.f[t], acc[db]);
+                if (low) acc[db] = mfma(__builtin_bit_cast(Frag, xy), low->f[t], acc[db]);
             }
     }
     static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) { return mfma(a, b, c); }
