@@ -144,7 +144,7 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
       scale      of q.k; dim ** -0.5 when not given          softcap    0: no cap
       slopes     float32 [heads], or None: no bias           causal     row i sees no key behind its position
       spans      int32 [batch or 1][rows][2]: the keys [first, last) of each row (key_spans makes them), or None: all
-      positions  int32 [rows] or [batch or 1][rows]; row i stands at i + keys - rows when not given
+      positions  int32 [rows] or [batch or 1][rows], within 2^30 of 0; row i stands at i + keys - rows when not given
     A row that sees no key comes out as noughts. Single tokens against long keys (rows = 1, one span each) are split over
     the GPU. Returns out [batch][rows][heads][dim], with return_lse also the log-sum-exp of w, float32
     [batch][heads][rows] (-inf for a row that sees none), which has no gradient; q, k and v have one."""
@@ -158,11 +158,11 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
         raise ValueError(f"span_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
     if not 1 <= dim <= MAX_DIM:
         raise ValueError(f"span_attention: at most {MAX_DIM} channels a head, got {dim}")
-    if not 0.0 <= softcap < 1e30:
-        raise ValueError(f"span_attention: softcap must not be negative, got {softcap}")
     scale = dim ** -0.5 if scale is None else float(scale)
     if not abs(scale) < 1e30:
         raise ValueError(f"span_attention: scale must be finite, got {scale}")
+    if softcap and not (1e-30 < softcap < 1e30 and abs(scale) / softcap < 1e30):
+        raise ValueError(f"span_attention: softcap is 0 or a positive number that the scale does not dwarf, got {softcap} with scale {scale}")
     if slopes is not None:
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,):
             raise ValueError(f"span_attention: slopes are float32 [{heads}], got {slopes.dtype} {tuple(slopes.shape)}")

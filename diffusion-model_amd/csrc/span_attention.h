@@ -341,6 +341,7 @@ __device__ __forceinline__ void settle(f32x16& x, f32x16& y) {
 struct Score {
     float pre, cap, inv, mul;            // inv: 1 / (cap log2 e), turns the result back into the tanh
     bool capped, plain;
+    float near16, near32;                // products below this, relative to the cap, go into the polynomials of apply
 
     __device__ __forceinline__ Score(const Dev& a) {
         capped = a.softcap > 0.f;
@@ -350,6 +351,9 @@ struct Score {
         // at scale 0 a number that makes every score nought and still keeps -infinity (a masked key) what it is
         pre = fmaxf(fabsf(capped ? a.scale / a.softcap : a.scale * kLog2e), 1e-37f);
         mul = plain ? pre : 1.f;
+        // their constants hold pre^6 and pre^10, which must not leave fp32's range: a scale of 1 / 128 and a cap of 50 do so for fp32
+        near16 = pre >= 1e-5f && pre <= 10.f && cap * pre <= 1e20f ? 0.5f : 0.f;
+        near32 = pre >= 1e-3f && near16 != 0.f ? 0.75f : 0.f;
     }
     // x into log2(e) u, where not plain
     template <typename T>
@@ -367,7 +371,7 @@ struct Score {
         float most = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[r]));
-        if (__all(most * pre < (exact ? 0.75f : 0.5f))) {
+        if (__all(most * pre < (exact ? near32 : near16))) {
             const float c0 = cap * pre, y = pre * pre, c1 = (exact ? -3.333306838e-01f : -3.332815933e-01f) * c0 * y;
             const float c2 = (exact ? 1.332652116e-01f : 1.320535960e-01f) * c0 * y * y;
             const float c3 = (exact ? -5.339025798e-02f : -4.475064100e-02f) * c0 * y * y * y;

@@ -5,6 +5,7 @@
 // running maximum and sum turn the scores into weights in one pass. With few rows (single tokens) the query heads that share
 // a key/value head are rows of one workgroup, and the keys are split over workgroups whose parts a second kernel joins.
 #include <algorithm>
+#include <cmath>
 
 #include "span_attention.h"
 
@@ -21,8 +22,9 @@ bool check_args(const ddpm_span_attention_args& a) {
     const auto fits = [&](const int64_t* s) { return s[0] % w == 0 && s[1] % w == 0 && s[2] % w == 0; };
     return (a.type == DDPM_F32 || a.type == DDPM_BF16 || a.type == DDPM_F16) && a.batch >= 0 && a.batch <= 65535 && a.nq >= 0 && a.nk >= 0 &&
            a.heads >= 1 && a.heads <= 65535 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0 && a.dim >= w &&
-           a.dim <= DDPM_SPAN_ATTENTION_MAX_DIM && a.dim % w == 0 && a.nq <= (1 << 30) && a.nk <= (1 << 30) && a.softcap >= 0.f &&
-           a.softcap <= 1e30f && a.scale >= -1e30f && a.scale <= 1e30f && fits(a.q_stride) && fits(a.k_stride) && fits(a.v_stride) &&
+           a.dim <= DDPM_SPAN_ATTENTION_MAX_DIM && a.dim % w == 0 && a.nq <= (1 << 30) && a.nk <= (1 << 30) &&
+           a.scale >= -1e30f && a.scale <= 1e30f && (a.softcap == 0.f || (a.softcap >= 1e-30f && a.softcap <= 1e30f &&
+           std::abs(a.scale) / static_cast<double>(a.softcap) <= 1e30)) && fits(a.q_stride) && fits(a.k_stride) && fits(a.v_stride) &&
            fits(a.out_stride) && fits_tile(a, a.k_stride) && fits_tile(a, a.v_stride);
 }
 

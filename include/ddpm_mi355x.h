@@ -430,7 +430,7 @@ typedef struct ddpm_span_attention_args {
     int32_t type;                    /* DDPM_F32, BF16, F16: of q, k, v, out and the gradients */
     int32_t batch, nq, nk, heads, kv_heads, dim;   /* heads a multiple of kv_heads, dim <= DDPM_SPAN_ATTENTION_MAX_DIM */
     int32_t causal;
-    float scale, softcap;            /* softcap >= 0 */
+    float scale, softcap;            /* softcap: 0, or 1e-30 ... 1e30 and |scale| / softcap <= 1e30 */
     const float* slopes;             /* [heads] or NULL */
     const int32_t* spans;            /* [batch or 1][nq][2]: first key, last key + 1; cut to [0, nk). NULL: all keys */
     const int32_t* positions;        /* [batch or 1][nq]; NULL: row i stands at i + nk - nq */

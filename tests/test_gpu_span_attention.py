@@ -127,6 +127,15 @@ def test_few_rows_against_many_keys(dtype, batch, nq, nk, heads, kv, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale,softcap,size", [(1e-3, 50.0, 50.0), (2e-5, 50.0, 350.0), (-2e-7, 1.0, 500.0), (1.0, 1e-4, 2e-3), (1.0, 1e-9, 0.0), (1e-30, 1e20, 100.0),
+                                                (1e-3, 50.0, 24.0), (2e-5, 50.0, 170.0), (-2e-7, 1.0, 240.0), (1.0, 1e-4, 1.1e-3), (1.0, 1e-3, 3.4e-3)])
+def test_scores_of_any_size_beside_the_cap(dtype, scale, softcap, size):
+    """Scores of about a third or a seventh of the cap (or none), made from very large and very small products."""
+    q, k, v, dout = _inputs(1, 70, 90, 2, 1, 32, dtype)
+    _check_all(q * size, k * size, v, dout, scale=scale, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nq,nk,heads,kv,dim", [(40, 1500, 4, 1, 64), (700, 700, 2, 2, 32), (1100, 600, 3, 1, 128), (2100, 90, 2, 1, 96), (1, 2000, 2, 2, 40)])
 def test_gradients_whose_work_is_dealt_out(dtype, nq, nk, heads, kv, dim):
     """Few blocks of rows (or keys) against many of the other: several workgroups share a block, and their sums are added up."""

@@ -135,7 +135,7 @@ def _span_args(at, **change):
 
 @pytest.mark.parametrize("change", [dict(type=3), dict(type=-1), dict(batch=-1), dict(batch=65536), dict(nq=-1), dict(nk=-1), dict(nk=(1 << 30) + 1),
                                     dict(heads=0), dict(heads=3, kv_heads=2), dict(kv_heads=0), dict(dim=0), dict(dim=10), dict(dim=132), dict(softcap=-1.0),
-                                    dict(softcap=math.nan), dict(scale=math.inf), dict(scale=math.nan), dict(q_stride=(1, 17)), dict(k_stride=(0, 2)),
+                                    dict(softcap=1e-31), dict(softcap=1e-3, scale=1e28), dict(softcap=math.nan), dict(scale=math.inf), dict(scale=math.nan), dict(q_stride=(1, 17)), dict(k_stride=(0, 2)),
                                     dict(v_stride=(2, 1)), dict(out_stride=(1, 3)), dict(type=1, dim=12), dict(type=1, q_stride=(1, 12))])
 def test_span_attention_refuses_sizes(change):
     keep, base = _aligned()
@@ -174,7 +174,8 @@ def test_span_attention_function_refuses():
     for args, how, error in (((q[0], k, k), {}, ValueError), ((q, k, k.half()), {}, TypeError), ((q.double(), k.double(), k.double()), {}, TypeError),
                              ((q, k, k[:, :8]), {}, ValueError), ((q, k[:1], k[:1]), {}, ValueError), ((q[:, :, :3], k, k), {}, ValueError),
                              ((torch.zeros(2, 6, 4, 136), torch.zeros(2, 9, 2, 136), torch.zeros(2, 9, 2, 136)), {}, ValueError),
-                             ((q, k, k), dict(softcap=-1.0), ValueError), ((q, k, k), dict(softcap=math.nan), ValueError),
+                             ((q, k, k), dict(softcap=-1.0), ValueError), ((q, k, k), dict(softcap=1e-31), ValueError),
+                             ((q, k, k), dict(softcap=1e-3, scale=1e28), ValueError), ((q, k, k), dict(softcap=math.nan), ValueError),
                              ((q, k, k), dict(scale=math.inf), ValueError), ((q, k, k), dict(slopes=torch.zeros(2)), ValueError),
                              ((q, k, k), dict(slopes=torch.zeros(4).double()), ValueError),
                              ((q, k, k), dict(slopes=torch.zeros(4).requires_grad_(True)), NotImplementedError),
