@@ -3,9 +3,10 @@
 // the gradient is the same turn by -theta. It stands beside the sinusoidal timestep embedding (embed.hip).
 //
 // Bound by HBM (x read once, y written once). A thread owns 16 bytes of channels of one token and loops over heads of q and
-// k, so that angles are formed once per token and channel and not once per head; 65536 tokens of
-// 16 + 4 bf16 heads of 128 channels and their gradient (1.34 GB) take 285 us, 4.7 TB/s, 95 % of a large copy's rate. Angles are formed in float64, in turns, and reduced there: a product in fp32 would be off by a whole radian at
-// position 10^7; the sine and cosine of the reduced angle are fp32 like everything else.
+// k, so that angles are formed once per token and channel and not once per head; 65536 tokens of 16 + 4 bf16 heads of 128
+// channels and their gradient (1.34 GB) take 284 us, 4.7 TB/s, 95 % of a large copy's rate. Angles are formed in float64, in
+// turns, and reduced there: a product in fp32 would be off by a whole radian at position 10^7; the sine and cosine of the
+// reduced angle are fp32 like everything else.
 #include <cmath>
 
 #include "common.h"

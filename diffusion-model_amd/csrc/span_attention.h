@@ -260,7 +260,8 @@ __device__ __forceinline__ f32x16 dot_from_lds(const T* tile, const T* own) {
 }
 
 // Rows of a tensor on their way to tiles in LDS. A tile's loads have one 64-bit address, which the wave keeps in scalar registers, and
-// 32-bit offsets of the lanes, which do not change from tile to tile (the host sees to it that kMaxTile rows span less than 2 GiB).
+// 32-bit unsigned offsets of the lanes, which do not change from tile to tile (the host sees to it that kMaxTile rows span less than
+// 2 GiB; no tile has more than twice as many).
 // Rows outside [lo, hi) read the nearest row inside: they are masked, and what memory holds behind a sequence is not looked
 // at. Chunks behind dim read the row's first one: their products with the noughts of an OwnRow are nought, and channels there
 // are not written. The loads have arrived behind the next arrived().
