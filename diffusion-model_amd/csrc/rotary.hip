@@ -175,7 +175,7 @@ extern "C" int ddpm_rotary(const ddpm_rotary_args* args, void* stream) {
     a.axes = r.axes;
     a.interleaved = r.interleaved != 0;
     a.total = static_cast<int64_t>(r.batch) * r.tokens;
-    DDPM_REQUIRE(a.total <= (int64_t(1) << 38) / r.dim);              // workgroups within 2^30
+    DDPM_REQUIRE(a.total <= ((int64_t(1) << 32) - 256) / r.dim * (wide ? width : 1));      // threads of a launch within 2^32
     a.sign = r.inverse ? -1.f : 1.f;
     a.positions = r.positions;
     a.position_type = r.position_type;

@@ -443,6 +443,10 @@ __device__ __forceinline__ int reg_row(int r, int half) { return 8 * (r >> 2) + 
 bool check_args(const ddpm_span_attention_args& a);
 bool fits_tile(const ddpm_span_attention_args& a, const int64_t* stride);      // rows of a tile within 32-bit offsets
 Dev dev_args(const ddpm_span_attention_args& a);
+// The grid holds 65535 entries of a batch; a longer one takes several launches, one behind the other, in the same workspace:
+// entries [first, first + kMaxBatch) of a.
+constexpr int kMaxBatch = 65535;
+ddpm_span_attention_args entries_from(const ddpm_span_attention_args& a, int first);
 
 // f(head size as a compile-time constant): dim rounded up to a multiple of 32
 template <typename F>

@@ -5,6 +5,8 @@
 // registers. That is 7 products for the 5 of a single kernel, whose dq would be added up with atomics in an order that changes
 // from call to call, and in fp32 memory that must be cleared before and converted behind. The gradient of a key/value head is
 // summed over the query heads that share it inside its workgroup.
+#include <algorithm>
+
 #include "span_attention.h"
 
 using ddpm::as_stream;
@@ -548,7 +550,10 @@ bool check_bwd(const ddpm_span_attention_args& a) {
 extern "C" int64_t ddpm_span_attention_bwd_workspace(const ddpm_span_attention_args* a) {
     if (!a || !check_bwd(*a)) return ddpm::fail_invalid("span attention sizes, type or strides");
     Work work;
-    return place(*a, nullptr, &work);
+    int64_t bytes = place(entries_from(*a, 0), nullptr, &work);
+    if (a->batch > kMaxBatch)            // the last launches, of fewer entries, may deal out their work
+        bytes = std::max(bytes, place(entries_from(*a, a->batch / kMaxBatch * kMaxBatch), nullptr, &work));
+    return bytes;
 }
 
 extern "C" int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* workspace, void* stream) {
@@ -560,11 +565,14 @@ extern "C" int ddpm_span_attention_bwd(const ddpm_span_attention_args* a, void* 
                           static_cast<const void*>(a->dk), static_cast<const void*>(a->dv), static_cast<const void*>(workspace)})
         DDPM_REQUIRE(ddpm::aligned16(p));
     DDPM_REQUIRE(a->nq == 0 || workspace);                // dk and dv of no rows are noughts, and need none
-    if (a->type == DDPM_F32)
-        launch<float>(*a, workspace, as_stream(stream));
-    else if (a->type == DDPM_BF16)
-        launch<__bf16>(*a, workspace, as_stream(stream));
-    else
-        launch<_Float16>(*a, workspace, as_stream(stream));
+    for (int64_t first = 0; first < a->batch; first += kMaxBatch) {
+        const ddpm_span_attention_args part = entries_from(*a, static_cast<int>(first));
+        if (a->type == DDPM_F32)
+            launch<float>(part, workspace, as_stream(stream));
+        else if (a->type == DDPM_BF16)
+            launch<__bf16>(part, workspace, as_stream(stream));
+        else
+            launch<_Float16>(part, workspace, as_stream(stream));
+    }
     return ddpm::check_launch("span attention backward");
 }

@@ -6,6 +6,7 @@
 // a key/value head are rows of one workgroup, and the keys are split over workgroups whose parts a second kernel joins.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "span_attention.h"
 
@@ -20,7 +21,7 @@ bool fits_tile(const ddpm_span_attention_args& a, const int64_t* stride) {
 bool check_args(const ddpm_span_attention_args& a) {
     const int w = a.type == DDPM_F32 ? 4 : 8;
     const auto fits = [&](const int64_t* s) { return s[0] % w == 0 && s[1] % w == 0 && s[2] % w == 0; };
-    return (a.type == DDPM_F32 || a.type == DDPM_BF16 || a.type == DDPM_F16) && a.batch >= 0 && a.batch <= 65535 && a.nq >= 0 && a.nk >= 0 &&
+    return (a.type == DDPM_F32 || a.type == DDPM_BF16 || a.type == DDPM_F16) && a.batch >= 0 && a.nq >= 0 && a.nk >= 0 &&
            a.heads >= 1 && a.heads <= 65535 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0 && a.dim >= w &&
            a.dim <= DDPM_SPAN_ATTENTION_MAX_DIM && a.dim % w == 0 && a.nq <= (1 << 30) && a.nk <= (1 << 30) &&
            a.scale >= -1e30f && a.scale <= 1e30f && (a.softcap == 0.f || (a.softcap >= 1e-30f && a.softcap <= 1e30f &&
@@ -63,6 +64,28 @@ Dev dev_args(const ddpm_span_attention_args& a) {
     d.sdk = strides(a.dk_stride);
     d.sdv = strides(a.dv_stride);
     return d;
+}
+
+ddpm_span_attention_args entries_from(const ddpm_span_attention_args& a, int first) {
+    ddpm_span_attention_args r = a;
+    const int64_t size = a.type == DDPM_F32 ? 4 : 2;
+    const auto move = [&](auto*& p, int64_t bytes) {
+        if (p) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(p) + first * bytes);
+    };
+    r.batch = std::min(a.batch - first, kMaxBatch);
+    move(r.spans, a.span_batch_stride * 4);
+    move(r.positions, a.position_batch_stride * 4);
+    move(r.q, a.q_stride[0] * size);
+    move(r.k, a.k_stride[0] * size);
+    move(r.v, a.v_stride[0] * size);
+    move(r.out, a.out_stride[0] * size);
+    move(r.out_low, a.out_stride[0] * size);
+    move(r.lse, static_cast<int64_t>(a.heads) * a.nq * 4);
+    move(r.dout, a.dout_stride[0] * size);
+    move(r.dq, a.dq_stride[0] * size);
+    move(r.dk, a.dk_stride[0] * size);
+    move(r.dv, a.dv_stride[0] * size);
+    return r;
 }
 
 }  // namespace span
@@ -329,7 +352,7 @@ void launch(const ddpm_span_attention_args& a, const Plan& plan, void* workspace
 extern "C" int64_t ddpm_span_attention_fwd_workspace(const ddpm_span_attention_args* a) {
     if (!a || !span::check_args(*a)) return ddpm::fail_invalid("span attention sizes, type or strides");
     if (a->batch == 0 || a->nq == 0) return 0;
-    const Plan plan = plan_of(*a);
+    const Plan plan = plan_of(*a);       // a batch that takes several launches is not split
     return plan.splits == 1 ? 0 : static_cast<int64_t>(plan.splits) * a->batch * a->heads * a->nq * (a->dim + 2) * 4;
 }
 
@@ -340,11 +363,14 @@ extern "C" int ddpm_span_attention_fwd(const ddpm_span_attention_args* a, void* 
     DDPM_REQUIRE(ddpm::aligned16(a->q) && ddpm::aligned16(a->k) && ddpm::aligned16(a->v) && ddpm::aligned16(a->out) && ddpm::aligned16(a->out_low));
     const Plan plan = plan_of(*a);
     DDPM_REQUIRE(plan.splits == 1 || (workspace && ddpm::aligned16(workspace)));
-    if (a->type == DDPM_F32)
-        launch<float>(*a, plan, workspace, as_stream(stream));
-    else if (a->type == DDPM_BF16)
-        launch<__bf16>(*a, plan, workspace, as_stream(stream));
-    else
-        launch<_Float16>(*a, plan, workspace, as_stream(stream));
+    for (int64_t first = 0; first < a->batch; first += span::kMaxBatch) {
+        const ddpm_span_attention_args part = span::entries_from(*a, static_cast<int>(first));
+        if (a->type == DDPM_F32)
+            launch<float>(part, plan, workspace, as_stream(stream));
+        else if (a->type == DDPM_BF16)
+            launch<__bf16>(part, plan, workspace, as_stream(stream));
+        else
+            launch<_Float16>(part, plan, workspace, as_stream(stream));
+    }
     return ddpm::check_launch("span attention forward");
 }

@@ -127,6 +127,16 @@ def test_few_rows_against_many_keys(dtype, batch, nq, nk, heads, kv, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_batches_of_more_entries_than_a_grid_holds(dtype):
+    b = 65535 + 9                                               # such as the frames of every pixel
+    q, k, v, dout = _inputs(b, 2, 3, 2, 1, 8, dtype)
+    g = torch.Generator().manual_seed(0)
+    ends = torch.sort(torch.randint(0, 4, (b, 2, 2), generator=g), -1).values.int().cuda()
+    positions = torch.randint(0, 9, (b, 2), generator=g).int().cuda()
+    _check_all(q, k, v, dout, spans=ends, positions=positions, slopes=_slopes(2))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("scale,softcap,size", [(1e-3, 50.0, 50.0), (2e-5, 50.0, 350.0), (-2e-7, 1.0, 500.0), (1.0, 1e-4, 2e-3), (1.0, 1e-9, 0.0), (1e-30, 1e20, 100.0),
                                                 (1e-3, 50.0, 24.0), (2e-5, 50.0, 170.0), (-2e-7, 1.0, 240.0), (1.0, 1e-4, 1.1e-3), (1.0, 1e-3, 3.4e-3)])
 def test_scores_of_any_size_beside_the_cap(dtype, scale, softcap, size):

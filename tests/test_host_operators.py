@@ -133,7 +133,7 @@ def _span_args(at, **change):
     return a
 
 
-@pytest.mark.parametrize("change", [dict(type=3), dict(type=-1), dict(batch=-1), dict(batch=65536), dict(nq=-1), dict(nk=-1), dict(nk=(1 << 30) + 1),
+@pytest.mark.parametrize("change", [dict(type=3), dict(type=-1), dict(batch=-1), dict(heads=65536, kv_heads=65536), dict(nq=-1), dict(nk=-1), dict(nk=(1 << 30) + 1),
                                     dict(heads=0), dict(heads=3, kv_heads=2), dict(kv_heads=0), dict(dim=0), dict(dim=10), dict(dim=132), dict(softcap=-1.0),
                                     dict(softcap=1e-31), dict(softcap=1e-3, scale=1e28), dict(softcap=math.nan), dict(scale=math.inf), dict(scale=math.nan), dict(q_stride=(1, 17)), dict(k_stride=(0, 2)),
                                     dict(v_stride=(2, 1)), dict(out_stride=(1, 3)), dict(type=1, dim=12), dict(type=1, q_stride=(1, 12))])
