@@ -90,7 +90,7 @@ def _run(entry, q, k, v, out, low, lse, how, gradient=_NO_GRADIENT):
               positions.stride(0) if positions is not None and positions.shape[0] > 1 else 0, x.data_ptr(), y.data_ptr(), v[0].data_ptr(),
               out[0].data_ptr(), _address(low), _address(lse), *q[1], *k[1], *v[1], *out[1], *gradient)
     size = getattr(lib(), entry + "_workspace")(a)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
+    workspace = x.new_empty(size, dtype=torch.uint8) if size > 0 else None
     call(entry, a, _address(workspace), stream_of(x.get_device()))
 
 
@@ -100,8 +100,8 @@ def _forward(q, k, v, how, with_lse, with_low=False):
     x = q[0]
     batch, rows, heads, dim = x.shape
     with on_gpu(x.get_device()):
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        lse = torch.empty((batch, heads, rows), dtype=torch.float32, device=x.device) if with_lse else None
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        lse = x.new_empty((batch, heads, rows), dtype=torch.float32) if with_lse else None
         low = torch.empty_like(out) if with_low and x.dtype != torch.float32 else None
         _run("ddpm_span_attention_fwd", q, k, v, _fit(out, width), low, lse, how)
     return x, k[0], v[0], out, low, lse
@@ -127,7 +127,7 @@ class _SpanAttention(torch.autograd.Function):
         width = _TYPES[q.dtype][1]
         with on_gpu(q.get_device()):
             dout, ds = _fit(dout, width)
-            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+            dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
             (_, qs), (_, ks) = _fit(dq, width), _fit(dk, width)
             gradient = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ds, *qs, *ks, *ks
             _run("ddpm_span_attention_bwd", _fit(q, width), _fit(k, width), _fit(v, width), _fit(out, width), low, lse,

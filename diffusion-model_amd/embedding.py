@@ -49,7 +49,7 @@ def _turn(tensors, positions, axes, base, interleaved, inverse):
     batch, tokens, _, dim = first.shape
     gpu = first.get_device()
     with on_gpu(gpu):
-        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in tensors]
+        outs = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in tensors]
         spare = 2 - len(tensors)                                # no k
         strides = [n for s in (tensors, outs) for n in (*(n for x in s for n in x.stride()[:3]), *(0,) * 3 * spare)]
         heads, *pointers = ((*values, *(0,) * spare) for values in ([x.shape[2] for x in tensors], map(_ptr, tensors), map(_ptr, outs)))
