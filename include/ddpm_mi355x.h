@@ -422,7 +422,8 @@ int ddpm_self_attention_infer(const float* x, int ldx, const float* wqkv_packed,
  * aligned, dim and the strides of q, k, v, out and the gradients multiples of 16 bytes (4 fp32, 8 16-bit elements), and the
  * row strides of k and v (backward: of q and dout too) not negative and below 32 MiB.
  * Arithmetic: fp32 inputs use the fp32 matrix instructions; 16-bit inputs have their weights and score gradients rounded
- * to 16 bits before the second product; scores, softmax statistics and sums are fp32 throughout.
+ * to 16 bits before the second product (score gradients enter dq as two 16-bit numbers); scores, softmax statistics and sums
+ * are fp32 throughout.
  * Stands beside ddpm_attention_fwd / _bwd (one head, no mask, second-iteration/unet.py:50-61).
  * ------------------------------------------------------------------------------------- */
 #define DDPM_SPAN_ATTENTION_MAX_DIM 128
