@@ -189,11 +189,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
             }
             // A score gradient enters as two 16-bit numbers. With one, dq would be off by its rounding, the rounding of dq and
             // what the forward call's rounded weights leave in D: 2.5e-3 of dq in bf16 where rounding dq alone leaves 1.66e-3,
-            // and 1.8e-3 so, for a quarter of this kernel's time (8192 rows and keys, 16 + 4 heads of 128: 806 us with one, 1031 with two).
+            // and 1.8e-3 so, for a quarter of this kernel's time (8192 rows and keys, 16 + 4 heads of 128: 806 us with one, 1004 to 1031 with two).
             const auto w = Ops<T>::pack(ds);
             if constexpr (sizeof(T) == 2) {
                 const auto low = Ops<T>::rest(ds, w);
+                // A wave with products to start goes before one that works on scores: 961 us for the 1004 of that call, 99 for 96
+                // with documents of 512; at 64 channels, and in the other two kernels, it makes no difference or costs.
+                if (DP > 64) __builtin_amdgcn_s_setprio(1);
                 Ops<T>::template spread<DP>(acc, k_now + kb * 32 * DP, w, &low);
+                if (DP > 64) __builtin_amdgcn_s_setprio(0);
             } else {
                 Ops<T>::template spread<DP>(acc, k_now + kb * 32 * DP, w);
             }
