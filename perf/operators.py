@@ -32,9 +32,9 @@ def _rotate(name, kind, batch, axes, sizes, heads, kv, dim, interleaved=False, t
 def listed():
     return [
         # attention over the 7x7 feature map at the bottom of a 28x28 network, one image: launch latency
-        _attend("attend 7x7 map one image", "fp32", 1, 49, 49, 4, 4, 32, "none"),
+        _attend("attend 7x7 map, one image", "fp32", 1, 49, 49, 4, 4, 32, "none"),
         # a training batch over 32x32 pixels in the network's own type, scores capped
-        _attend("attend 32x32 pixels training", "fp32", 32, 1024, 1024, 4, 4, 32, "none", cap=30.0),
+        _attend("attend 32x32 pixels, training", "fp32", 32, 1024, 1024, 4, 4, 32, "none", cap=30.0),
         # label or text tokens in front of 45x45 pixels: the prefix sees itself, the pixels follow one by one; odd length
         _attend("attend prefix and pixels", "bf16", 4, 2125, 2125, 16, 16, 64, "prefix", cap=50.0),
         # images of different sizes packed into one sequence, shared key/value heads, distance bias
@@ -42,19 +42,19 @@ def listed():
         # a 128x128 image at once, inference
         _attend("attend 128x128 pixels", "bf16", 1, 16384, 16384, 8, 8, 128, "none", train=False),
         # single tokens of a ragged batch against their key/value buffers
-        _attend("attend one token batch", "bf16", 32, 1, 8192, 32, 8, 128, "lengths", slopes=True, train=False),
+        _attend("attend one token, batch", "bf16", 32, 1, 8192, 32, 8, 128, "lengths", slopes=True, train=False),
         # two single tokens against long buffers, an odd head size: few rows, a long axis
-        _attend("attend one token long", "fp16", 2, 1, 65536, 16, 2, 80, "lengths", cap=50.0, train=False),
+        _attend("attend one token, long", "fp16", 2, 1, 65536, 16, 2, 80, "lengths", cap=50.0, train=False),
         # positions of one new token of each sequence of a batch, far along: launch latency
         _rotate("rotate one token", "bf16", 16, "32,48,48", "1,1,1", 32, 8, 128, offset=100000),
         # positions of 16 frames of 64x64 with their gradient, shared key heads
-        _rotate("rotate 16 frames training", "bf16", 1, "32,48,48", "16,64,64", 16, 4, 128, train=True),
+        _rotate("rotate 16 frames, training", "bf16", 1, "32,48,48", "16,64,64", 16, 4, 128, train=True),
         # the clipped optimizer step of the smallest network of the tests: many tiny tensors
-        {"name": "clipped step tiny network", "op": "step", "unet": 8, "emb": 16, "max_norm": 1.0},
+        {"name": "clipped step, tiny network", "op": "step", "unet": 8, "emb": 16, "max_norm": 1.0},
         # the clipped optimizer step of the full second-iteration network
-        {"name": "clipped step full network", "op": "step", "unet": 64, "emb": 128, "max_norm": 1.0},
+        {"name": "clipped step, full network", "op": "step", "unet": 64, "emb": 128, "max_norm": 1.0},
         # clipping alone over a large list of tensors of two types, ragged sizes
-        {"name": "clip 400 tensors two types", "op": "clip", "tensors": 400, "largest": 1 << 21, "type": "mixed", "max_norm": 1.0},
+        {"name": "clip 400 tensors, two types", "op": "clip", "tensors": 400, "largest": 1 << 21, "type": "mixed", "max_norm": 1.0},
     ]
 
 
