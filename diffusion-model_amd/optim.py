@@ -190,7 +190,7 @@ class Adam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = []
+        work, entries = [], {}                                  # entries: of each parameter, so far
         for group in self.param_groups:
             by_step = {}
             for p in group["params"]:
@@ -210,11 +210,13 @@ class Adam(torch.optim.Optimizer):
                     st["step"] = torch.tensor(0.0, dtype=torch.float32)
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                by_step.setdefault(int(st["step"].item()) + 1, []).append((p, g, st["exp_avg"], st["exp_avg_sq"]))
-            work += [(group, step, items) for step, items in by_step.items()]
+                # a parameter that a group lists twice takes two steps, one launch behind the other: in one they would race
+                entries[p] = entries.get(p, 0) + 1
+                by_step.setdefault(int(st["step"].item()) + entries[p], []).append((p, g, st["exp_avg"], st["exp_avg_sq"]))
+            work += [(group, step, items) for step, items in sorted(by_step.items())]
         norm = None
         if self.max_grad_norm is not None and work:
-            norm = _Norm("Adam", [t[1] for _, _, items in work for t in items], self.max_grad_norm, 2.0)
+            norm = _Norm("Adam", list({t[0]: t[1] for _, _, items in work for t in items}.values()), self.max_grad_norm, 2.0)
             self.grad_norm = norm.state[0]
         for group, step, items in work:
             with on_gpu(items[0][0].get_device()):

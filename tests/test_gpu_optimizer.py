@@ -1,0 +1,46 @@
+"""`optim.Adam` in calls that a training loop may make beside the ordinary one. All comparisons are bit for bit: the same updates are
+made in another way."""
+import warnings
+
+import pytest
+import torch
+
+from diffusion_model_amd import optim
+
+pytestmark = pytest.mark.gpu
+SIZES = [1, 5, 2047, 2048, 2049, 5000]
+
+
+def _params(seed):
+    g = torch.Generator().manual_seed(seed)
+    out = [torch.nn.Parameter(torch.randn(n, generator=g).cuda()) for n in SIZES]
+    for p in out:
+        p.grad = torch.randn(p.shape, generator=g).cuda()
+    return out
+
+
+def _adam(params, **how):
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")                         # torch warns of parameters listed twice
+        return optim.Adam(params, lr=1e-2, **how)
+
+
+def _equal(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("max_grad_norm", [None, 0.3])
+def test_a_parameter_listed_twice_takes_two_steps(max_grad_norm):
+    """As two steps of an optimizer that lists it once, with the same gradients."""
+    a, b = _params(1), _params(1)
+    twice, once = _adam(a + a[2:], max_grad_norm=max_grad_norm), _adam(b, max_grad_norm=max_grad_norm)
+    twice.step()
+    once.step()
+    if max_grad_norm is not None:
+        assert torch.equal(twice.grad_norm, once.grad_norm)
+    first = [p.detach().clone() for p in b[:2]]
+    once.step()
+    assert _equal(a[:2], first) and _equal(a[2:], b[2:])
+    for p, q in zip(a[2:], b[2:]):
+        assert float(twice.state[p]["step"]) == 2.0
+        assert all(torch.equal(twice.state[p][k], once.state[q][k]) for k in ("exp_avg", "exp_avg_sq"))
