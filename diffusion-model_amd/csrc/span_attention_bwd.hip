@@ -485,9 +485,9 @@ int parts_for(int64_t blocks, int64_t wanted, int64_t tiles, int least) {
 // Two workgroups a compute unit fill the chip; spans load them unevenly, and then four are better. dk and dv of 8192 packed tokens in
 // documents of 340, 4 key/value heads shared by 16, are 256 blocks: 1056 us with a workgroup each, 542 with two, 304 with four,
 // 285 with eight; where all rows see all keys 1692 us with one, 1178 with two, 1192 with four.
-int parts_of(const ddpm_span_attention_args& a) {
+int parts_of(const ddpm_span_attention_args& a, bool spans) {
     const int64_t blocks = (static_cast<int64_t>(a.nk) + kRows - 1) / kRows * a.kv_heads * a.batch;
-    return parts_for(blocks, a.spans ? 1024 : 512, (static_cast<int64_t>(a.nq) + 31) / 32 * (a.heads / a.kv_heads), 8);
+    return parts_for(blocks, spans ? 1024 : 512, (static_cast<int64_t>(a.nq) + 31) / 32 * (a.heads / a.kv_heads), 8);
 }
 int q_parts_of(const ddpm_span_attention_args& a) {
     const int64_t blocks = (static_cast<int64_t>(a.nq) + kRows - 1) / kRows * a.heads * a.batch;
@@ -496,7 +496,8 @@ int q_parts_of(const ddpm_span_attention_args& a) {
 
 int groups_of(int nq) { return (nq + kRows - 1) / kRows * 4; }
 
-// Places the parts of Work in a workspace, and returns its size.
+// Places the parts of Work in a workspace, and returns its size: that of a call with spans, which has the more parts, so that one workspace
+// serves all calls of the same sizes and type.
 int64_t place(const ddpm_span_attention_args& a, void* workspace, Work* w) {
     w->groups = groups_of(a.nq);
     const int64_t rows = static_cast<int64_t>(a.batch) * w->groups, heads = rows * a.heads;
@@ -515,8 +516,8 @@ int64_t place(const ddpm_span_attention_args& a, void* workspace, Work* w) {
     w->q_sums = reinterpret_cast<float*>(at);
     if (w->q_parts > 1) at += static_cast<int64_t>(w->q_parts) * a.batch * a.nq * a.heads * a.dim * 4;
     w->sums = reinterpret_cast<float*>(at);
-    w->parts = parts_of(a);
-    if (w->parts > 1) at += static_cast<int64_t>(w->parts) * 2 * a.batch * a.nk * a.kv_heads * a.dim * 4;
+    w->parts = parts_of(a, a.spans != nullptr);
+    if (const int most = parts_of(a, true); most > 1) at += static_cast<int64_t>(most) * 2 * a.batch * a.nk * a.kv_heads * a.dim * 4;
     return at - static_cast<char*>(workspace);
 }
 
