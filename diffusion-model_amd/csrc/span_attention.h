@@ -336,6 +336,79 @@ __device__ __forceinline__ void settle(f32x16& x, f32x16& y) {
         asm volatile("s_nop 11" : "+v"(x), "+v"(y));
 }
 
+// ---- keys that no row sees ---------------------------------------------------------------------------------------------
+// A masked key has weight nought, but nought times what its row of v (for dq, of k) holds is nought for finite numbers alone. Keys outside
+// of all that a workgroup's rows see are not fetched; the ones in between that none of them sees, as behind each of several padded
+// documents, are made noughts in LDS. Where the rows see neighbouring or overlapping spans, one after the other, there are none, which
+// takes some comparisons of a lane; elsewhere a search, and in a tile with such keys a barrier: 8192 rows, 16 + 4 heads of 128, bf16, in
+// documents of 340 padded to 352 take 64 us (forward) and 329 (with the gradient) for the 61 and 321 without, of 352 the same as without.
+struct Gaps {
+    static constexpr int kRows = kThreads / 2;
+    int lo[kRows], hi[kRows];            // of the workgroup's rows
+    int from[kRows], to[kRows];          // gaps
+
+    // before a barrier: the rows of this wave, whose lane halves hold the same
+    __device__ __forceinline__ void tell(const Row& row) {
+        if ((threadIdx.x & 32) == 0) {
+            const int x = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+            lo[x] = row.lo;
+            hi[x] = row.hi;
+        }
+    }
+    // behind it, for all of the workgroup: how many gaps there are below key `top`. Every wave searches by itself.
+    __device__ __forceinline__ int find(int top) {
+        // A gap begins at the end of a span that is in no span, and ends where the next one begins. Most ends are in the next row's span, or are
+        // its end too; those that are not are looked at one by one. A row that sees none has lo = INT_MAX, hi = 0.
+        const int lane = threadIdx.x & 63;
+        int l[2], h[2];
+        unsigned long long ends[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = lane + 64 * i;
+            l[i] = lo[x];
+            h[i] = hi[x];
+            ends[i] = __ballot(h[i] != 0 && h[i] < top && !(x + 1 < kRows && lo[x + 1] <= h[i] && hi[x + 1] >= h[i]));
+        }
+        int n = 0;
+        while (ends[0] | ends[1]) {
+            const int end = ends[0] ? __builtin_amdgcn_readlane(h[0], __builtin_ctzll(ends[0])) : __builtin_amdgcn_readlane(h[1], __builtin_ctzll(ends[1]));
+            bool inside = false;
+            int next = INT32_MAX;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                ends[i] &= ~__ballot(h[i] == end);
+                inside |= l[i] <= end && h[i] > end;
+                if (l[i] > end) next = min(next, l[i]);
+            }
+            if (__any(inside)) continue;
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) next = min(next, __shfl_xor(next, d));
+            if (threadIdx.x == 0) {
+                from[n] = end;
+                to[n] = next;
+            }
+            ++n;
+        }
+        if (n > 0) __syncthreads();
+        return n;
+    }
+    // nought into the rows of two tiles of keys j0 ... that are in a gap; `n` is the same for the workgroup
+    template <typename T, int DP, int TILE>
+    __device__ __forceinline__ void clear(int n, int j0, T* x, T* y) const {
+        constexpr int kChunks = DP / Ops<T>::W;
+        typedef typename Ops<T>::Frag Frag;
+        bool any = false;
+        for (int g = 0; g < n; ++g) {
+            const int first = max(from[g] - j0, 0), last = min(to[g] - j0, TILE);
+            if (first >= last) continue;
+            any = true;
+            for (int c = first * kChunks + static_cast<int>(threadIdx.x); c < last * kChunks; c += kThreads)
+                reinterpret_cast<Frag*>(x)[c] = reinterpret_cast<Frag*>(y)[c] = Frag{};
+        }
+        if (any) __syncthreads();
+    }
+};
+
 // ---- scores ------------------------------------------------------------------------------------------------------------
 // From x = |scale| / scale q.k to log2(e) w. Where there is neither cap nor bias that is a product with a constant, which goes into the
 // exponential's argument as exp2(x * mul - maximum), one operation for both; elsewhere log2(e) w is formed first, and mul is 1 there.

@@ -73,6 +73,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     constexpr bool kGain = __is_same(T, _Float16);
     __shared__ __attribute__((aligned(1024))) T k_even[kTile * DP], k_odd[kTile * DP], v_even[kTile * DP], v_odd[kTile * DP];
     __shared__ int bounds[2][4];
+    __shared__ Gaps gaps;
 
     const Place id = place_of();
     const int parts = SPLIT ? work.q_parts : 1, part = SPLIT ? id.x % parts : 0;
@@ -100,6 +101,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
         bounds[0][wave] = wlo;
         bounds[1][wave] = whi;
     }
+    if (a.spans) gaps.tell(row);
     const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
     OwnRow<T, DP> q, dout;
     q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
@@ -124,6 +126,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    const int unseen = a.spans ? gaps.find(hi) : 0;      // without spans a row sees all keys from the first on
     const int first = lo < hi ? lo / kTile + part : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;      // every parts-th tile
 
     const Score score(a);
@@ -137,13 +140,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
         ks.load(k_even, first * kTile, a.dim);
         vs.load(v_even, first * kTile, a.dim);
     }
-    const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
+    const auto step = [&](int t, T* k_now, T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
         arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
         if (t + parts < last) {
             ks.load(k_next, j0 + parts * kTile, a.dim);
             vs.load(v_next, j0 + parts * kTile, a.dim);
         }
+        if (unseen) gaps.template clear<T, DP, kTile>(unseen, j0, k_now, v_now);
         if (j0 + kTile <= wlo || j0 >= whi) return;
         const bool whole = __all(row.lo <= j0 && row.hi >= j0 + kTile);
 #pragma unroll
@@ -215,6 +219,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DP <= 256 ? 2 : 1) void dq_ke
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) settle<T>(acc[db]);
     if (!real) return;
+    if (row.hi == 0) {                   // sees none, whatever the others see
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+    }
     const float f = kGain ? inverse_gain(gain) * a.scale : a.scale;
     if (SPLIT)
         write_row<float, DP>(work.q_sums + (((static_cast<int64_t>(part) * gridDim.z + b) * a.nq + i) * a.heads + head) * a.dim, acc, f, a.dim);

@@ -129,6 +129,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
     constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
     __shared__ __attribute__((aligned(1024))) T k_even[kTile * DP], k_odd[kTile * DP], v_even[kTile * DP], v_odd[kTile * DP];
     __shared__ int bounds[2][4];
+    __shared__ Gaps gaps;
 
     // x: row blocks (the last first: under causal order they have most to do), and with SPLIT the parts of the keys beside them
     const Place id = place_of();
@@ -149,12 +150,14 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         bounds[0][wave] = wlo;
         bounds[1][wave] = whi;
     }
+    if (a.spans) gaps.tell(row);
     OwnRow<T, DP> q;
     q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
     if (a.scale < 0.f) q.negate();       // Score counts on a factor that is positive
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    const int unseen = a.spans ? gaps.find(hi) : 0;      // without spans a row sees all keys from the first on
 
     int first = lo < hi ? lo / kTile : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;   // tiles
     if (SPLIT) {
@@ -175,13 +178,14 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         ks.load(k_even, first * kTile, a.dim);
         vs.load(v_even, first * kTile, a.dim);
     }
-    const auto step = [&](int t, const T* k_now, const T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
+    const auto step = [&](int t, T* k_now, T* v_now, T* k_next, T* v_next) __attribute__((always_inline)) {
         arrived();                       // tile t is here, tile t - 1 is done with
         const int j0 = t * kTile;
         if (t + 1 < last) {
             ks.load(k_next, j0 + kTile, a.dim);
             vs.load(v_next, j0 + kTile, a.dim);
         }
+        if (unseen) gaps.template clear<T, DP, kTile>(unseen, j0, k_now, v_now);
         if (j0 + kTile <= wlo || j0 >= whi) return;                 // nothing here for this wave's rows
         f32x16 s[kBlocks];
 #pragma unroll
@@ -261,7 +265,12 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         return;
     }
     if (a.lse && half == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top - Ops<T>::kShift + log2f(sum)) * kLn2;
+    // no weight, no output: nought times a sum of noughts would be NaN where another row sees a value that is not finite
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f) {
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+    }
     const int64_t out = b * a.so.batch + i * a.so.row + head * a.so.head;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
@@ -325,6 +334,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Dev a, const Parts part
 #pragma unroll
     for (int g = 1; g < 8; ++g) acc += group_acc[g][threadIdx.x];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f) acc = f32x4{};
     const float o[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
     write_out<T>(a, b * a.so.batch + i * a.so.row + head * a.so.head + c, o);
 }

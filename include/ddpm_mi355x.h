@@ -416,8 +416,9 @@ int ddpm_self_attention_infer(const float* x, int ldx, const float* wqkv_packed,
  *   w = u - slopes[h] * |position_i - j|      for the keys that row i sees, first_i <= j < last_i (and j <= position_i when causal)
  *   out_i = sum_j softmax_j(w) v_j            lse_i = log sum_j exp(w)
  * A row that sees no key (or whose keys all have weight nought) has out = 0, lse = -infinity and no gradient. Keys that no
- * row sees have gradient 0, and what q, k and v hold there does not matter; a value that is not finite at a key that some row sees
- * may reach other rows of that batch entry, as a product with weight nought does.
+ * row sees have gradient 0. What k and v hold at such keys, between spans too, and q and dout in such rows does not matter. A value
+ * that is not finite at a key that some row sees may reach other rows of that batch entry that see a key, and one of q or dout in a
+ * row that sees a key the gradients of other keys, as a product with weight nought does.
  * Element (b, n, h, c) of a tensor lies at its base + b*stride[0] + n*stride[1] + h*stride[2] + c. Bases must be 16-byte
  * aligned, dim and the strides of q, k, v, out and the gradients multiples of 16 bytes (4 fp32, 8 16-bit elements), and the
  * row strides of k and v (backward: of q and dout too) not negative and below 32 MiB.
