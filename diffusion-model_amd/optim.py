@@ -184,6 +184,15 @@ class Adam(torch.optim.Optimizer):
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None        # norm of the gradients of the last step (0-dim, on the device) with max_grad_norm
 
+    # torch's optimizers take their groups and state along when copied or pickled, and nothing else
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "grad_norm": self.grad_norm}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.setdefault("max_grad_norm", None)         # pickled before there was one
+        self.__dict__.setdefault("grad_norm", None)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -1,5 +1,7 @@
 """`optim.Adam` in calls that a training loop may make beside the ordinary one. All comparisons are bit for bit: the same updates are
 made in another way."""
+import copy
+import pickle
 import warnings
 
 import pytest
@@ -44,3 +46,19 @@ def test_a_parameter_listed_twice_takes_two_steps(max_grad_norm):
     for p, q in zip(a[2:], b[2:]):
         assert float(twice.state[p]["step"]) == 2.0
         assert all(torch.equal(twice.state[p][k], once.state[q][k]) for k in ("exp_avg", "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("max_grad_norm", [None, 0.3])
+@pytest.mark.parametrize("through", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
+def test_a_copied_optimizer_goes_on_as_the_first(max_grad_norm, through):
+    a = _params(2)
+    grads = [p.grad for p in a]
+    first = _adam(a, max_grad_norm=max_grad_norm)
+    first.step()
+    second = through(first)
+    b = second.param_groups[0]["params"]
+    for p, q, g in zip(a, b, grads):
+        p.grad, q.grad = g, g.clone()
+    first.step()
+    second.step()
+    assert _equal(a, b) and (max_grad_norm is None or torch.equal(first.grad_norm, second.grad_norm))
