@@ -9,6 +9,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DDPM_LIB") or os.path.join(_HERE, "libddpm_mi355x.so")   # DDPM_LIB: diagnostic builds
@@ -235,6 +236,13 @@ _ALREADY = contextlib.nullcontext()
 def on_gpu(gpu):
     """with on_gpu(index): the GPU is the current one. Nothing to do where it is already, which it mostly is."""
     return _ALREADY if torch.cuda.current_device() == gpu else torch.cuda.device(gpu)
+
+
+def refuse_tangents(what, tensors):
+    """Raises for tensors of forward-mode differentiation, whose tangents a kernel would drop without a word. Outside of a dual level,
+    where no tensor has one, the level alone is looked at."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors if x is not None):
+        raise NotImplementedError(f"{what}: no forward-mode derivatives")
 
 
 def call(name, *args):

@@ -4,7 +4,7 @@ windows, causal order), with its gradient. It stands beside the UNet's own self-
 head, every pixel sees every pixel) for networks over tokens of images, video and text."""
 import torch
 
-from ._lib import SpanAttentionArgs, call, lib, on_gpu, packer, stream_of
+from ._lib import SpanAttentionArgs, call, lib, on_gpu, packer, refuse_tangents, stream_of
 
 _TYPES = {torch.float32: (0, 4), torch.bfloat16: (1, 8), torch.float16: (2, 8)}      # DDPM_* code, elements of 16 bytes
 MAX_DIM = 128
@@ -178,6 +178,7 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
         if positions.dtype != torch.int32 or tuple(positions.shape) not in ((batch, rows), (1, rows)):
             raise ValueError(f"span_attention: positions are int32 [{batch} or 1][{rows}], got {positions.dtype} {tuple(positions.shape)}")
         positions = positions.contiguous()
+    refuse_tangents("span_attention", (q, k, v, slopes))
     if not all(x.is_cuda and x.device == q.device for x in (q, k, v, slopes, spans, positions) if x is not None):
         raise RuntimeError("span_attention runs on the MI355X only: all tensors must be on one GPU")
     spare = -dim % _TYPES[q.dtype][1]

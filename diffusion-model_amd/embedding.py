@@ -5,7 +5,7 @@ import ctypes as C
 import torch
 import torch.nn as nn
 
-from ._lib import RotaryArgs, call, on_gpu, packer, stream_of
+from ._lib import RotaryArgs, call, on_gpu, packer, refuse_tangents, stream_of
 
 
 class SinusoidalTimeEmbedding(nn.Module):
@@ -101,6 +101,7 @@ def rotary(q, k, positions, axes, base=10000.0, interleaved=False):
     batch, tokens = q.shape[:2]
     if tuple(positions.shape) not in ((tokens, len(axes)), (batch, tokens, len(axes)), (1, tokens, len(axes))):
         raise ValueError(f"rotary: positions are [tokens][axes] or [batch][tokens][axes] for {(batch, tokens, len(axes))}, got {tuple(positions.shape)}")
+    refuse_tangents("rotary", (*tensors, positions))
     if not all(x.is_cuda and x.device == q.device for x in (*tensors, positions)):
         raise RuntimeError("rotary runs on the MI355X only: q, k and positions must be on one GPU")
     positions = positions.contiguous()

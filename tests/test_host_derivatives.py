@@ -1,0 +1,32 @@
+"""Derivatives that the operators for networks over tokens do not have are refused, not dropped; the refusals come before the GPU is
+asked for."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from diffusion_model_amd.attention import span_attention
+from diffusion_model_amd.embedding import rotary
+
+
+def _dual(*shape):
+    return forward_ad.make_dual(torch.zeros(shape), torch.ones(shape))
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_is_refused(no_grad):
+    q, k = torch.zeros(1, 6, 4, 16), torch.zeros(1, 9, 2, 16)
+    pos = torch.zeros(6, 1)
+    with torch.set_grad_enabled(not no_grad), forward_ad.dual_level():
+        dq, dk = _dual(1, 6, 4, 16), _dual(1, 9, 2, 16)
+        for args, how in (((dq, k, k), {}), ((q, dk, k), {}), ((q, k, dk), {}), ((q, k, k), dict(slopes=_dual(4)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                span_attention(*args, **how)
+        for args in ((dq, None, pos, (16,)), (q, dq, pos, (16,)), (q, None, _dual(6, 1), (16,))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                rotary(*args)
+        with pytest.raises(RuntimeError, match="one GPU"):       # a level alone refuses nothing
+            span_attention(q, k, k)
+        with pytest.raises(RuntimeError, match="one GPU"):
+            rotary(q, None, pos, (16,))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda x: span_attention(x, k, k), (q,), (q,))
