@@ -52,7 +52,7 @@ class SpanAttentionArgs(C.Structure):
                 ("position_batch_stride", I64), ("q", P), ("k", P), ("v", P), ("out", P), ("out_low", P), ("lse", P)] + \
                [(n, I64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
                [(n, P) for n in ("dout", "dq", "dk", "dv")] + \
-               [(n, I64 * 3) for n in ("dout_stride", "dq_stride", "dk_stride", "dv_stride")]
+               [(n, I64 * 3) for n in ("dout_stride", "dq_stride", "dk_stride", "dv_stride")] + [("lse_near", P)]
 
 
 def packer(structure):

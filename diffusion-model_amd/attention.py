@@ -79,7 +79,7 @@ _pack = packer(SpanAttentionArgs)
 _NO_GRADIENT = (0,) * 16
 
 
-def _run(entry, q, k, v, out, low, lse, how, gradient=_NO_GRADIENT):
+def _run(entry, q, k, v, out, low, lse, near, how, gradient=_NO_GRADIENT):
     """q, k, v, out: (tensor, strides). Runs on the current GPU, the tensors' own."""
     scale, softcap, slopes, spans, positions, causal = how
     x, y = q[0], k[0]
@@ -88,13 +88,13 @@ def _run(entry, q, k, v, out, low, lse, how, gradient=_NO_GRADIENT):
     a = _pack(_TYPES[x.dtype][0], batch, rows, keys, heads, kv_heads, dim, causal, scale, softcap, _address(slopes), _address(spans),
               _address(positions), spans.stride(0) if spans is not None and spans.shape[0] > 1 else 0,
               positions.stride(0) if positions is not None and positions.shape[0] > 1 else 0, x.data_ptr(), y.data_ptr(), v[0].data_ptr(),
-              out[0].data_ptr(), _address(low), _address(lse), *q[1], *k[1], *v[1], *out[1], *gradient)
+              out[0].data_ptr(), _address(low), _address(lse), *q[1], *k[1], *v[1], *out[1], *gradient, _address(near))
     size = getattr(lib(), entry + "_workspace")(a)
     workspace = x.new_empty(size, dtype=torch.uint8) if size > 0 else None
     call(entry, a, _address(workspace), stream_of(x.get_device()))
 
 
-def _forward(q, k, v, how, with_lse, with_low=False):
+def _forward(q, k, v, how, with_lse, training=False):
     width = _TYPES[q.dtype][1]
     q, k, v = _fit(q, width), _fit(k, width), _fit(v, width)
     x = q[0]
@@ -102,16 +102,17 @@ def _forward(q, k, v, how, with_lse, with_low=False):
     with on_gpu(x.get_device()):
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
         lse = x.new_empty((batch, heads, rows), dtype=torch.float32) if with_lse else None
-        low = torch.empty_like(out) if with_low and x.dtype != torch.float32 else None
-        _run("ddpm_span_attention_fwd", q, k, v, _fit(out, width), low, lse, how)
-    return x, k[0], v[0], out, low, lse
+        low = torch.empty_like(out) if training and x.dtype != torch.float32 else None
+        near = torch.empty_like(lse) if training and how[2] is not None else None       # without a bias it is lse
+        _run("ddpm_span_attention_fwd", q, k, v, _fit(out, width), low, lse, near, how)
+    return x, k[0], v[0], out, low, lse, near
 
 
 class _SpanAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, softcap, slopes, spans, positions, causal):
-        q, k, v, out, low, lse = _forward(q, k, v, (scale, softcap, slopes, spans, positions, causal), True, True)
-        ctx.save_for_backward(q, k, v, out, low, lse, slopes, spans, positions)
+        q, k, v, out, low, lse, near = _forward(q, k, v, (scale, softcap, slopes, spans, positions, causal), True, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, near, slopes, spans, positions)
         ctx.how = scale, softcap, causal
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -122,7 +123,7 @@ class _SpanAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return (None,) * 9
-        q, k, v, out, low, lse, slopes, spans, positions = ctx.saved_tensors
+        q, k, v, out, low, lse, near, slopes, spans, positions = ctx.saved_tensors
         scale, softcap, causal = ctx.how
         width = _TYPES[q.dtype][1]
         with on_gpu(q.get_device()):
@@ -130,7 +131,7 @@ class _SpanAttention(torch.autograd.Function):
             dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
             (_, qs), (_, ks) = _fit(dq, width), _fit(dk, width)
             gradient = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ds, *qs, *ks, *ks
-            _run("ddpm_span_attention_bwd", _fit(q, width), _fit(k, width), _fit(v, width), _fit(out, width), low, lse,
+            _run("ddpm_span_attention_bwd", _fit(q, width), _fit(k, width), _fit(v, width), _fit(out, width), low, lse, near,
                  (scale, softcap, slopes, spans, positions, causal), gradient)
         return dq, dk, dv, None, None, None, None, None, None
 
@@ -187,7 +188,7 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v)):
         out, lse = _SpanAttention.apply(q, k, v, scale, float(softcap), slopes, spans, positions, bool(causal))
     else:
-        _, _, _, out, _, lse = _forward(q, k, v, (scale, float(softcap), slopes, spans, positions, bool(causal)), return_lse)
+        _, _, _, out, _, lse, _ = _forward(q, k, v, (scale, float(softcap), slopes, spans, positions, bool(causal)), return_lse)
     if spare:
         out = out[..., :dim].contiguous()
     return (out, lse) if return_lse else out

@@ -40,7 +40,7 @@ struct Dev {
     int64_t span_batch, position_batch;
     const void *q, *k, *v;
     void *out, *out_low;
-    float* lse;
+    float *lse, *lse_near;
     Strides sq, sk, sv, so;
     const void* dout;
     void *dq, *dk, *dv;
@@ -48,13 +48,20 @@ struct Dev {
 };
 
 // ---- what a row sees -----------------------------------------------------------------------------------------------
+// The bias counts from the nearest key that the row sees: -slope |pos - j| with pos moved there differs from the one with the row's position by
+// the same number for all of them, which the softmax does not notice. Far from all its keys (a million positions at a slope of 0.5) the
+// full bias would take the scores' last bits: one step of fp32 is 0.06 there.
 struct Row {
-    int lo, hi, pos;                     // keys [lo, hi); lo = INT_MAX, hi = 0: none
+    int lo, hi, pos;                     // keys [lo, hi); lo = INT_MAX, hi = 0: none; position, moved to the nearest key
 };
+
+__device__ __forceinline__ int position_of(const Dev& a, int b, int i) {
+    return a.positions ? a.positions[b * a.position_batch + i] : i + a.nk - a.nq;
+}
 
 __device__ __forceinline__ Row row_of(const Dev& a, int b, int i) {
     Row r;
-    r.pos = a.positions ? a.positions[b * a.position_batch + i] : i + a.nk - a.nq;
+    r.pos = position_of(a, b, i);
     r.lo = 0;
     r.hi = a.nk;
     if (a.spans) {
@@ -66,8 +73,18 @@ __device__ __forceinline__ Row row_of(const Dev& a, int b, int i) {
     if (r.hi <= r.lo) {
         r.lo = INT32_MAX;
         r.hi = 0;
+    } else {
+        r.pos = min(max(r.pos, r.lo), r.hi - 1);
     }
     return r;
+}
+
+// what the move left out of the bias of all keys: lse = lse_near - it
+__device__ __forceinline__ float left_out(const Dev& a, int b, int i, const Row& row, int head) {
+    if (!a.slopes || row.hi == 0) return 0.f;
+    const int at = position_of(a, b, i);
+    const unsigned way = at < row.pos ? static_cast<unsigned>(row.pos) - static_cast<unsigned>(at) : static_cast<unsigned>(at) - static_cast<unsigned>(row.pos);
+    return a.slopes[head] * static_cast<float>(way);
 }
 
 __device__ __forceinline__ Row no_row() { return {INT32_MAX, 0, 0}; }

@@ -51,6 +51,7 @@ Dev dev_args(const ddpm_span_attention_args& a) {
     d.out = a.out;
     d.out_low = a.out_low;
     d.lse = a.lse;
+    d.lse_near = a.lse_near;
     d.sq = strides(a.q_stride);
     d.sk = strides(a.k_stride);
     d.sv = strides(a.v_stride);
@@ -81,6 +82,7 @@ ddpm_span_attention_args entries_from(const ddpm_span_attention_args& a, int fir
     move(r.out, a.out_stride[0] * size);
     move(r.out_low, a.out_stride[0] * size);
     move(r.lse, static_cast<int64_t>(a.heads) * a.nq * 4);
+    move(r.lse_near, static_cast<int64_t>(a.heads) * a.nq * 4);
     move(r.dout, a.dout_stride[0] * size);
     move(r.dq, a.dq_stride[0] * size);
     move(r.dk, a.dk_stride[0] * size);
@@ -115,6 +117,11 @@ Plan plan_of(const ddpm_span_attention_args& a) {
     p.splits = all > 0 && all < 512 ? static_cast<int>(std::min<int64_t>((512 + all - 1) / all, tiles / 4)) : 1;
     p.splits = std::max(1, std::min(p.splits, kMaxSplits));
     return p;
+}
+
+__device__ __forceinline__ void write_lse(const Dev& a, int64_t at, float lse, int b, int i, const Row& row, int head) {
+    if (a.lse_near) a.lse_near[at] = lse;
+    if (a.lse) a.lse[at] = lse - left_out(a, b, i, row, head);
 }
 
 struct Parts {                           // of a split call: per part and row the sum before division, its maximum and weight sum
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         }
         return;
     }
-    if (a.lse && half == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top - Ops<T>::kShift + log2f(sum)) * kLn2;
+    if (half == 0) write_lse(a, at, sum == 0.f ? -INFINITY : (top - Ops<T>::kShift + log2f(sum)) * kLn2, b, i, row, head);
     // no weight, no output: nought times a sum of noughts would be NaN where another row sees a value that is not finite
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (sum == 0.f) {
@@ -329,7 +336,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Dev a, const Parts part
     const int64_t bh = at / a.nq;
     const int head = static_cast<int>(bh % a.heads);
     const int64_t b = bh / a.heads;
-    if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2;
+    if (threadIdx.x == 0) write_lse(a, at, sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2, static_cast<int>(b), i, row_of(a, static_cast<int>(b), i), head);
     if (c >= a.dim) return;
 #pragma unroll
     for (int g = 1; g < 8; ++g) acc += group_acc[g][threadIdx.x];

@@ -447,6 +447,9 @@ typedef struct ddpm_span_attention_args {
     const void* dout;
     void *dq, *dk, *dv;
     int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+    float* lse_near;                 /* like lse, of w with distances counted from the nearest key that the row sees: written by the
+                                        forward call and read by the backward one; NULL: the gradients' weights come from lse, and are off
+                                        by 2^-24 |lse| of themselves where a bias makes that large */
 } ddpm_span_attention_args;
 
 /* Bytes of workspace (16-byte aligned, contents unspecified afterwards) of the two calls; negative for bad arguments.
