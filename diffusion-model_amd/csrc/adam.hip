@@ -114,6 +114,7 @@ int adam_step(int ntensors, float* const* params, const float* const* grads, flo
         DDPM_REQUIRE(numel[i] >= 0 && numel[i] <= ddpm::kLongestTensor);
         DDPM_REQUIRE(numel[i] == 0 || (params[i] && grads[i] && exp_avg[i] && exp_avg_sq[i]));
     }
+    DDPM_REQUIRE(ddpm::chunks_fit(ntensors, numel, kTensorsPerLaunch, kChunk));
     for (int t0 = 0; t0 < ntensors; t0 += kTensorsPerLaunch) {
         AdamBatch b;
         const int cnt = ntensors - t0 < kTensorsPerLaunch ? ntensors - t0 : kTensorsPerLaunch;

@@ -178,6 +178,9 @@ __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const List l, const
 
 bool known_type(int t) { return t == DDPM_F32 || t == DDPM_BF16 || t == DDPM_F16; }
 
+// no launch's chunks pass 32 bits
+static_assert(kTensors * (ddpm::kLongestTensor / kChunk) + kMaxBlocks <= INT32_MAX, "chunks of a launch");
+
 int check_list(int ntensors, const void* const* grads, const int64_t* numel, const int32_t* types) {
     for (int i = 0; i < ntensors; ++i) {
         DDPM_REQUIRE(known_type(types[i]));

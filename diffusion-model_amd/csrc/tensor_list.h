@@ -27,7 +27,19 @@ __device__ __forceinline__ int tensor_of_chunk(const ChunkMap<N>& m, int chunk) 
     return lo;
 }
 
-// Longest tensor of a list: more than any GPU holds, and few enough chunks that a launch's count stays within 32 bits.
+// Longest tensor of a list, in elements.
 constexpr int64_t kLongestTensor = int64_t(1) << 36;
+
+// Does the number of chunks of every launch over `per_launch` tensors stay within 32 bits, a grid's step past the last one included? For
+// checked lengths.
+inline bool chunks_fit(int ntensors, const int64_t* numel, int per_launch, int64_t chunk) {
+    int64_t chunks = 0;
+    for (int i = 0; i < ntensors; ++i) {
+        if (i % per_launch == 0) chunks = 0;
+        chunks += (numel[i] + chunk - 1) / chunk;
+        if (chunks > INT32_MAX - 65536) return false;
+    }
+    return true;
+}
 
 }  // namespace ddpm
