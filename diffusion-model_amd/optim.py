@@ -47,10 +47,10 @@ def _distinct(what, pointers, sizes):
 
 class _Norm:
     """The gradients of one call as the C arrays of the norm and clipping entry points, and the norm itself:
-    `state` holds [norm, factor] on the device. They must be contiguous; where the caller has their pointers and sizes already
-    it hands them in."""
+    `state` holds [norm, factor] on the device. They must be contiguous, and different ones where `written` says that they will be
+    scaled in place; where the caller has their pointers and sizes already it hands them in."""
 
-    def __init__(self, what, grads, max_norm, norm_type, pointers=None, sizes=None):
+    def __init__(self, what, grads, max_norm, norm_type, pointers=None, sizes=None, written=False):
         if norm_type not in _NORMS:
             raise NotImplementedError(f"{what} (HIP): norm_type must be 2 or inf, got {norm_type}")
         if not max_norm >= 0.0:
@@ -62,6 +62,7 @@ class _Norm:
         self.n = len(grads)
         if pointers is None:
             pointers, sizes = list(map(_ptr, grads)), list(map(_numel, grads))
+        if written:
             _distinct(what, pointers, sizes)
         (self.pointers, a), (self.numel, b), (self.types, c) = _array("Q", pointers), _array("q", sizes), _array("i", types)
         self._owners = (a, b, c)
@@ -94,20 +95,22 @@ def _gradients(what, parameters):
 @torch.no_grad()
 def grad_norm(parameters, norm_type=2.0):
     """Norm of all gradients of `parameters` together (a 0-dim fp32 tensor on their GPU): the 2-norm, summed in float64
-    in a fixed order, or with norm_type=inf the largest magnitude. The gradients stay as they are."""
+    in a fixed order, or with norm_type=inf the largest magnitude. The gradients stay as they are; one that several parameters
+    share counts for each of them."""
     _, grads = _gradients("grad_norm", parameters)
     return _Norm("grad_norm", grads, math.inf, float(norm_type)).state[0] if grads else torch.tensor(0.0)
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """torch.nn.utils.clip_grad_norm_ over fp32, bf16 and fp16 gradients on one GPU: scales all of them in place by
     min(1, max_norm / (norm + 1e-6)) and returns the norm before (0-dim fp32, on the device; nothing waits for it unless
-    error_if_nonfinite is set). A norm that is not a number makes every gradient NaN, as there."""
+    error_if_nonfinite is set). A norm that is not a number makes every gradient NaN, as there. Norms other than 2 and inf, and a
+    gradient given twice, are refused; `foreach` chooses between torch's implementations, and here there is one."""
     grads, dense = _gradients("clip_grad_norm_", parameters)
     if not grads:
         return torch.tensor(0.0)
-    norm = _Norm("clip_grad_norm_", dense, max_norm, float(norm_type))
+    norm = _Norm("clip_grad_norm_", dense, max_norm, float(norm_type), written=True)
     if error_if_nonfinite and not math.isfinite(norm.state[0].item()):
         raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
     with on_gpu(norm.device):

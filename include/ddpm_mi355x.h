@@ -181,7 +181,7 @@ int ddpm_adam_step(int ntensors, float* const* params, const float* const* grads
 /* Norm of a list of gradients taken together, and clipping by it: what a training loop puts between backward and
  * optimizer step (loss.backward(); optimizer.step(), first-iteration/main.py:83-84; the reference does not clip). Host
  * arrays of ntensors device pointers (aligned to their elements), element counts and DDPM_F32 / BF16 / F16 codes, consumed
- * before the call returns; a gradient must not be listed twice.
+ * before the call returns; ddpm_clip_grads must not be given a gradient twice.
  *   ddpm_grad_norm: state[0] = norm (DDPM_NORM_2: square root of the float64 sum of squares; DDPM_NORM_MAX: largest
  *     magnitude; NaN when a gradient is), state[1] = min(1, max_norm / (norm + 1e-6)), two device floats. The same
  *     gradients give the same bits. workspace: ddpm_grad_norm_workspace_doubles(ntensors) doubles.

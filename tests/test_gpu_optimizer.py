@@ -62,3 +62,34 @@ def test_a_copied_optimizer_goes_on_as_the_first(max_grad_norm, through):
     first.step()
     second.step()
     assert _equal(a, b) and (max_grad_norm is None or torch.equal(first.grad_norm, second.grad_norm))
+
+
+def test_a_gradient_that_parameters_share():
+    """The norm counts it for each of them, and so does the clipped step, which reads gradients alone; scaling it twice is refused."""
+    a, b = _params(3), _params(3)
+    a[4].grad = a[5].grad[:2049]                                # the same memory, of two sizes
+    b[4].grad = a[4].grad.clone()
+    a.append(torch.nn.Parameter(a[5].detach().clone()))
+    a[-1].grad = a[5].grad
+    b.append(torch.nn.Parameter(a[5].detach().clone()))
+    b[-1].grad = a[5].grad.clone()
+    want = optim.grad_norm(b)
+    assert torch.equal(optim.grad_norm(a), want)
+    assert float(want) == pytest.approx(float(torch.cat([p.grad.double() for p in a]).norm()), rel=2.0 ** -23)
+    with pytest.raises(ValueError, match="twice"):
+        optim.clip_grad_norm_(a, 0.3)
+    for params in (a, b):
+        opt = _adam(params, max_grad_norm=0.3)
+        opt.step()
+        assert torch.equal(opt.grad_norm, want)
+    assert _equal(a, b)
+
+
+def test_clipping_takes_the_arguments_of_torch():
+    tol = sum(SIZES) * 2.0 ** -24                               # what adding up that many squares in fp32 is off by at most
+    for foreach in (None, False, True):
+        a, b = _params(4), _params(4)
+        got = optim.clip_grad_norm_(a, 0.5, 2.0, False, foreach)
+        want = torch.nn.utils.clip_grad_norm_(b, 0.5, 2.0, False, foreach)
+        assert float(got) == pytest.approx(float(want), rel=tol)
+        assert all(torch.allclose(p.grad, q.grad, rtol=tol, atol=0) for p, q in zip(a, b))
