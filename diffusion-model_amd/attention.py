@@ -167,7 +167,7 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
     if slopes is not None:
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,):
             raise ValueError(f"span_attention: slopes are float32 [{heads}], got {slopes.dtype} {tuple(slopes.shape)}")
-        if slopes.requires_grad:
+        if slopes.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("span_attention: slopes have no gradient")
         slopes = slopes.contiguous()
     if spans is not None:

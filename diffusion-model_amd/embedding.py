@@ -96,7 +96,7 @@ def rotary(q, k, positions, axes, base=10000.0, interleaved=False):
         raise ValueError(f"rotary: axes are 1 to 4 even channel counts of together at most {q.shape[3]}, got {axes}")
     if q.shape[3] > 512:
         raise ValueError(f"rotary: at most 512 channels, got {q.shape[3]}")
-    if positions.dtype not in _POSITION_TYPES or positions.requires_grad:
+    if positions.dtype not in _POSITION_TYPES or positions.requires_grad and torch.is_grad_enabled():
         raise TypeError(f"rotary: positions are int32, int64 or float32 without a gradient, got {positions.dtype}")
     batch, tokens = q.shape[:2]
     if tuple(positions.shape) not in ((tokens, len(axes)), (batch, tokens, len(axes)), (1, tokens, len(axes))):

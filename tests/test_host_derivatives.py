@@ -30,3 +30,18 @@ def test_forward_mode_is_refused(no_grad):
             rotary(q, None, pos, (16,))
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda x: span_attention(x, k, k), (q,), (q,))
+
+
+def test_slopes_and_positions_of_a_model_serve_without_gradients():
+    """Learned ones have no gradient here, which matters where gradients are recorded."""
+    q, k = torch.zeros(1, 6, 4, 16), torch.zeros(1, 9, 2, 16)
+    slopes, pos = torch.zeros(4, requires_grad=True), torch.zeros(6, 1, requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        span_attention(q, k, k, slopes=slopes)
+    with pytest.raises(TypeError):
+        rotary(q, None, pos, (16,))
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="one GPU"):       # asked last
+            span_attention(q, k, k, slopes=slopes)
+        with pytest.raises(RuntimeError, match="one GPU"):
+            rotary(q, None, pos, (16,))
