@@ -15,15 +15,16 @@ using ddpm::as_stream;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 176;             // 22 bytes of kernel arguments each, below 4 KiB together
+constexpr int kTensors = 176;             // 20 bytes of kernel arguments each, below 4 KiB together
 constexpr int64_t kChunk = 8192;          // elements: 8 (fp32) or 4 (16-bit) loads of 16 bytes per thread in flight
 constexpr int kMaxBlocks = 2048;          // 8 workgroups per compute unit; also the partial results a launch leaves
 
+// Lengths and types share a word. With the types as bytes, the compiler took the address of a byte, kernel arguments + t, as the base of the
+// scalar load of p[t] as well, and 7 t as its offset: scalar loads drop the low two bits of each.
 struct List {
     ddpm::ChunkMap<kTensors> map;
     void* p[kTensors];
-    int64_t n[kTensors];
-    uint8_t type[kTensors];
+    int64_t length_type[kTensors];        // 4 n + type
 };
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -111,14 +112,14 @@ struct Chunk {
 // f<T>(first element, elements) of every chunk of this workgroup
 template <typename F>
 __device__ __forceinline__ void each_chunk(const List& l, F f) {
-    const int chunks = l.map.first[l.map.count];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    for (int c = blockIdx.x; c < l.map.chunks; c += gridDim.x) {
         const int t = ddpm::tensor_of_chunk(l.map, c);
         const int64_t begin = static_cast<int64_t>(c - l.map.first[t]) * kChunk;
-        const int n = static_cast<int>(kChunk < l.n[t] - begin ? kChunk : l.n[t] - begin);
-        if (l.type[t] == DDPM_F32)
+        const int64_t left = (l.length_type[t] >> 2) - begin;
+        const int n = static_cast<int>(kChunk < left ? kChunk : left), type = static_cast<int>(l.length_type[t] & 3);
+        if (type == DDPM_F32)
             f(static_cast<float*>(l.p[t]) + begin, n);
-        else if (l.type[t] == DDPM_BF16)
+        else if (type == DDPM_BF16)
             f(static_cast<__bf16*>(l.p[t]) + begin, n);
         else
             f(static_cast<_Float16*>(l.p[t]) + begin, n);
@@ -193,22 +194,14 @@ int check_list(int ntensors, const void* const* grads, const int64_t* numel, con
 // tensors t0, t0 + 1, ... of the list, as many as one launch takes
 void fill(List& l, int t0, int ntensors, const void* const* grads, const int64_t* numel, const int32_t* types) {
     const int cnt = ntensors - t0 < kTensors ? ntensors - t0 : kTensors;
-    int32_t chunks = 0;
-    l.map.count = cnt;
-    l.map.first[0] = 0;
+    ddpm::map_chunks(l.map, numel + t0, cnt, kChunk);
     for (int i = 0; i < cnt; ++i) {
         l.p[i] = const_cast<void*>(grads[t0 + i]);
-        l.n[i] = numel[t0 + i];
-        l.type[i] = static_cast<uint8_t>(types[t0 + i]);
-        chunks += static_cast<int32_t>((numel[t0 + i] + kChunk - 1) / kChunk);
-        l.map.first[i + 1] = chunks;
+        l.length_type[i] = 4 * numel[t0 + i] + types[t0 + i];
     }
 }
 
-int blocks_of(const List& l) {
-    const int chunks = l.map.first[l.map.count];
-    return chunks < kMaxBlocks ? chunks : kMaxBlocks;
-}
+int blocks_of(const List& l) { return l.map.chunks < kMaxBlocks ? l.map.chunks : kMaxBlocks; }
 
 }  // namespace
 

@@ -6,25 +6,34 @@
 
 namespace ddpm {
 
-// first[t] = number of chunks before tensor t; first[count] = chunks in all. Tensors without elements own no chunk.
+// first[t] = number of chunks before tensor t, INT32_MAX behind the last tensor. Tensors without elements own no chunk.
 template <int N>
 struct ChunkMap {
-    int32_t count;
-    int32_t first[N + 1];
+    int32_t chunks;                      // in all
+    int32_t first[N];
 };
 
-// the tensor that owns `chunk` (uniform over the workgroup)
+// the map of tensors of these lengths, `count` of them
+template <int N>
+void map_chunks(ChunkMap<N>& m, const int64_t* numel, int count, int64_t chunk) {
+    m.chunks = 0;
+    for (int i = 0; i < N; ++i) {
+        m.first[i] = i < count ? m.chunks : INT32_MAX;
+        if (i < count) m.chunks += static_cast<int32_t>((numel[i] + chunk - 1) / chunk);
+    }
+}
+
+// The tensor that owns `chunk` (uniform over the workgroup): the last one that begins at it or before. A wave looks at all of them at once; a
+// search by halves waits for up to eight scalar loads, one behind the other.
 template <int N>
 __device__ __forceinline__ int tensor_of_chunk(const ChunkMap<N>& m, int chunk) {
-    int lo = 0, hi = m.count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (m.first[mid] <= chunk)
-            lo = mid;
-        else
-            hi = mid;
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < N; i += 64) {
+        const int t = i + static_cast<int>(threadIdx.x & 63);
+        before += __popcll(__ballot(t < N && m.first[t] <= chunk));
     }
-    return lo;
+    return before - 1;
 }
 
 // Longest tensor of a list, in elements.
