@@ -22,8 +22,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;            // 4 waves
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// running maximum before the first key: finite, so that its difference from -infinity (a masked score) is one
-constexpr float kNoMax = -1e30f;
+// Running maximum before the first key: finite, so that its difference from -infinity (a masked score) is one, and below any finite score but
+// fp32's lowest ones, so that a row's first score takes its place.
+constexpr float kNoMax = -3e38f;
 constexpr int kMaxTile = 64;             // rows of a tile, at most
 
 struct Strides {

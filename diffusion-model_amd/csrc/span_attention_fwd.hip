@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         last = begin + static_cast<int>(static_cast<int64_t>(n) * (part + 1) / parts.splits);
     }
 
-    const Score score(a);
+    Score score(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
 
     f32x16 acc[DP / 32] = {};
@@ -232,6 +232,14 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
             sum *= f;
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) acc[db] *= f;
+            // A score enters its exponential as a product that is not rounded, and `top` is one that is: past 2^20 what the rounding left
+            // would be a factor of its own, and overflow. From there on scores are rounded first.
+            if (score.plain && __any(fabsf(top) > 1048576.f && top != kNoMax)) {
+#pragma unroll
+                for (int kb = 0; kb < kBlocks; ++kb) s[kb] *= score.mul;
+                score.plain = false;
+                score.mul = 1.f;
+            }
         }
         const float shift = Ops<T>::kShift - top;
 #pragma unroll
