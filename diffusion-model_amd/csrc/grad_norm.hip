@@ -63,7 +63,8 @@ __device__ __forceinline__ double take(double acc, float g) {
 
 // The elements of a chunk [p, p + n) on their way through a thread's registers: all of its loads are in flight before the first is
 // used, behind a tensor's end too. A last chunk of 8191 elements taken one by one took longer than the rest of a launch:
-// 26.5 us for the norm of 133 tensors of 62 MB and 26.2 us for their clipping, 17.5 and 21.9 us so.
+// 26.5 us for the norm of 133 tensors of 62 MB and 26.2 us for their clipping, 17.5 and 21.9 us so. 133 ragged tensors of 59 MB take 13.7 and
+// 18.9 us with their bases on 16-byte boundaries, 13.8 and 19.2 with none of them.
 template <typename T>
 struct Chunk {
     typedef typename Wide<T>::type V;

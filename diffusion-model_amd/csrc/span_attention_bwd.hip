@@ -2,7 +2,7 @@
 //   D_i = sum_c dout_ic out_ic,  p_ij = exp(w_ij - lse_i),  dp_ij = dout_i . v_j,  ds_ij = scale (du/dt)_ij p_ij (dp_ij - D_i)
 //   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
 // in two kernels, each of which recomputes the scores: dq walks over keys with rows in registers, dk and dv over rows with keys in
-// registers. That is 7 products for the 5 of a single kernel, whose dq would be added up with atomics in an order that changes
+// registers. That is 7 products (for 16-bit types 8, as score gradients enter dq in two parts) for the 5 of a single kernel, whose dq would be added up with atomics in an order that changes
 // from call to call, and in fp32 memory that must be cleared before and converted behind. The gradient of a key/value head is
 // summed over the query heads that share it inside its workgroup.
 #include <algorithm>
@@ -67,7 +67,8 @@ __device__ __forceinline__ void write_row(T* out, const f32x16* acc, float f, in
 // dq. A workgroup of 4 waves takes 128 rows of one head, 32 a wave, and walks over the keys that any of them sees; where there are few
 // rows and many keys several workgroups take a tile in turn each (SPLIT), and a last kernel adds up their sums. It also leaves what the
 // other kernel has to know of the rows. Up to 32 channels there is room for three waves on a SIMD: 32 x 1024 rows and keys, 4 heads, fp32 take
-// 555 us (the whole gradient) with them, 566 with two.
+// 555 us (the whole gradient) with them, 566 with two. fp32 above 64 channels has one wave: 4 x 1024 rows, 8 heads of 128 take 546 us so, and
+// 855 with two, whose registers spill; at 96 channels both take 426.
 template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(kThreads, DP <= 32 ? 3 : sizeof(T) * DP <= 256 ? 2 : 1) void dq_kernel(const Dev a, const Work work) {
     constexpr int kTile = Ops<T>::kTile, kBlocks = kTile / 32;
@@ -433,6 +434,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
                 }
             }
             if constexpr (kGain) ds *= gain * kUnshift;
+            // 16-bit types round weights and score gradients once: dk and dv are off by 2.4e-3 of themselves (bf16), 1.4 times what rounding
+            // them alone leaves; a second part, as in dq, would cost two more products.
             Ops<T>::template spread<DP, kFresh>(dv, do_now + g * 32 * DP, Ops<T>::pack(s));
             if (kFresh) __builtin_amdgcn_sched_barrier(0);
             Ops<T>::template spread<DP, kFresh>(dk, q_now + g * 32 * DP, Ops<T>::pack(ds));

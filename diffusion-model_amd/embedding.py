@@ -80,8 +80,8 @@ def rotary(q, k, positions, axes, base=10000.0, interleaved=False):
     """Rotary positions of queries [batch][tokens][heads][dim] and keys (own head count, or None), as new tensors; one launch,
     with a gradient for q and k. Axis a owns axes[a] channels (even), consecutive from channel 0; its pair i is turned by
     positions[..., a] * base^(-2 i / axes[a]); further channels pass. Pairs are (i, axes[a]/2 + i), or with interleaved
-    (2 i, 2 i + 1). positions: [tokens][len(axes)], or [batch or 1][tokens][len(axes)]; int32, int64 or float32, integers
-    of any size: angles are formed in float64. q and k: float32, bfloat16 or float16, any strides.
+    (2 i, 2 i + 1). positions: [tokens][len(axes)], or [batch or 1][tokens][len(axes)]; int32, int64 or float32, angles are
+    formed in float64, off by 2^-51 radian for each unit of the position. q and k: float32, bfloat16 or float16, any strides.
     Returns (q, k), or q alone when k is None."""
     tensors = (q,) if k is None else (q, k)
     axes = tuple(int(d) for d in axes)

@@ -236,7 +236,7 @@ int ddpm_sinusoidal_embedding(const void* t, int t_is_float, int batch, int emb_
 /* Rotary positions with several axes (time, height, width; one for a plain sequence): pair i of the axis_dim[a] channels
  * of axis a is turned by positions[token][a] * base^(-2 i / axis_dim[a]); the axes own consecutive channels from 0 on, and
  * channels behind the last axis pass unchanged. A pair is (i, axis_dim/2 + i) within its axis, or (2 i, 2 i + 1) with
- * interleaved != 0. inverse != 0 turns back: the gradient of the forward call. Angles are formed and reduced in float64.
+ * interleaved != 0. inverse != 0 turns back: the gradient of the forward call. Angles are formed and reduced in float64 (off by 2^-51 of the position).
  * One or two tensors (queries and keys of one sequence, own head counts) with the same positions; element (b, n, h, c) of
  * tensor i lies at x[i] + b*x_stride[i][0] + n*x_stride[i][1] + h*x_stride[i][2] + c, so that a channel slice of a fused
  * projection serves; out must not overlap x. positions: [batch or 1][tokens][axes], DDPM_I32, I64 or F32;
@@ -425,7 +425,7 @@ int ddpm_self_attention_infer(const float* x, int ldx, const float* wqkv_packed,
  * Arithmetic: fp32 inputs use the fp32 matrix instructions; 16-bit inputs have their weights and score gradients rounded
  * to 16 bits before the second product (score gradients enter dq as two 16-bit numbers); scores, softmax statistics and sums
  * are fp32 throughout. The backward call's weights are exp(w - lse): fp32 roundings of numbers of the size of w make them off by up
- * to 2^-22 |w| of themselves, so that scores in the millions leave gradients few right digits (the forward call compares scores with the
+ * to 2^-21 |w| of themselves, so that scores in the millions leave gradients few right digits (the forward call compares scores with the
  * row's largest and keeps its own).
  * Stands beside ddpm_attention_fwd / _bwd (one head, no mask, second-iteration/unet.py:50-61).
  * ------------------------------------------------------------------------------------- */
