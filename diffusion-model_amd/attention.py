@@ -149,7 +149,7 @@ def span_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, spans=None,
     A row that sees no key comes out as noughts. Single tokens against long keys (rows = 1, one span each) are split over
     the GPU. Returns out [batch][rows][heads][dim], with return_lse also the log-sum-exp of w, float32
     [batch][heads][rows] (-inf for a row that sees none), which has no gradient; q, k and v have one, whose weights exp(w - lse)
-    are off by up to 2^-21 |w| of themselves: scores in the millions leave it few right digits."""
+    are off by up to 2^-21 |w| of themselves: scores in the millions leave it few right digits, from some 10^8 on none."""
     for name, x in (("q", q), ("k", k), ("v", v)):
         if x.dim() != 4:
             raise ValueError(f"span_attention: {name} is [batch][tokens][heads][dim], got {tuple(x.shape)}")

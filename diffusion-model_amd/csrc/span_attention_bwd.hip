@@ -103,7 +103,8 @@ __global__ __launch_bounds__(kThreads, DP <= 32 ? 3 : sizeof(T) * DP <= 256 ? 2 
         bounds[0][wave] = wlo;
         bounds[1][wave] = whi;
     }
-    if (a.spans) gaps.tell(row);
+    const bool apart = a.spans && a.nq > 1;              // without spans a row sees all keys from the first on
+    if (apart) gaps.tell(row);
     const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.nq + i;
     OwnRow<T, DP> q, dout;
     q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(kThreads, DP <= 32 ? 3 : sizeof(T) * DP <= 256 ? 2 
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
-    const int unseen = a.spans ? gaps.find(hi) : 0;      // without spans a row sees all keys from the first on
+    const int unseen = apart ? gaps.find(hi) : 0;
     const int first = lo < hi ? lo / kTile + part : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;      // every parts-th tile
 
     const Score score(a);

@@ -157,14 +157,15 @@ __global__ __launch_bounds__(kThreads, 2) void fwd_kernel(const Dev a, const int
         bounds[0][wave] = wlo;
         bounds[1][wave] = whi;
     }
-    if (a.spans) gaps.tell(row);
+    const bool apart = a.spans && a.nq > 1;              // without spans a row sees all keys from the first on
+    if (apart) gaps.tell(row);
     OwnRow<T, DP> q;
     q.load(real ? static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.row + head * a.sq.head : nullptr, a.dim);
     if (a.scale < 0.f) q.negate();       // Score counts on a factor that is positive
     __syncthreads();
     const int lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
     const int hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
-    const int unseen = a.spans ? gaps.find(hi) : 0;      // without spans a row sees all keys from the first on
+    const int unseen = apart ? gaps.find(hi) : 0;
 
     int first = lo < hi ? lo / kTile : 0, last = lo < hi ? (hi + kTile - 1) / kTile : 0;   // tiles
     if (SPLIT) {
@@ -346,7 +347,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Dev a, const Parts part
     const int64_t bh = at / a.nq;
     const int head = static_cast<int>(bh % a.heads);
     const int64_t b = bh / a.heads;
-    if (threadIdx.x == 0) write_lse(a, at, sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2, static_cast<int>(b), i, row_of(a, static_cast<int>(b), i), head);
+    if ((a.lse || a.lse_near) && threadIdx.x == 0)
+        write_lse(a, at, sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2, static_cast<int>(b), i, row_of(a, static_cast<int>(b), i), head);
     if (c >= a.dim) return;
 #pragma unroll
     for (int g = 1; g < 8; ++g) acc += group_acc[g][threadIdx.x];

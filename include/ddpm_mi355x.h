@@ -425,8 +425,8 @@ int ddpm_self_attention_infer(const float* x, int ldx, const float* wqkv_packed,
  * Arithmetic: fp32 inputs use the fp32 matrix instructions; 16-bit inputs have their weights and score gradients rounded
  * to 16 bits before the second product (score gradients enter dq as two 16-bit numbers); scores, softmax statistics and sums
  * are fp32 throughout. The backward call's weights are exp(w - lse): fp32 roundings of numbers of the size of w make them off by up
- * to 2^-21 |w| of themselves, so that scores in the millions leave gradients few right digits (the forward call compares scores with the
- * row's largest and keeps its own).
+ * to 2^-21 |w| of themselves, so that scores in the millions leave gradients few right digits, and from some 10^8 on none, nor finite ones
+ * (the forward call compares scores with the row's largest and keeps its digits).
  * Stands beside ddpm_attention_fwd / _bwd (one head, no mask, second-iteration/unet.py:50-61).
  * ------------------------------------------------------------------------------------- */
 #define DDPM_SPAN_ATTENTION_MAX_DIM 128

@@ -111,3 +111,34 @@ def test_rows_that_see_none_are_nought_whatever_the_others_see(dtype, nq, nk):
     out, lse, dq, _, _ = _run((q, k, v), dout, spans=spans)
     assert (out[:, ::2] == 0).all() and (dq[:, ::2] == 0).all() and (lse[..., ::2] == -math.inf).all()
     assert out[:, 1::2, 0].isnan().all() and not out[:, 1::2, 1, 2].isfinite().any()
+
+
+def test_replayed_graph_finds_the_gaps_of_the_spans_it_meets():
+    """Padded documents with a bias, forward and gradient, captured once; spans and inputs change between replays, and NaN stands at
+    what is not seen."""
+    n = 192
+    q, k, v, dout = (_rand((1, n, h, 64), BF16, s) for s, h in enumerate((4, 2, 2, 4)))
+    spans = _spans("padded", n).cuda()
+    slopes = torch.full((4,), 0.01, device="cuda")
+    step = lambda: _run((q, k, v), dout, spans=spans, slopes=slopes)          # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i, kind in enumerate(("scattered", "padded causal", "two ends", "padded")):
+        spans.copy_(_spans(kind, n))
+        keys, rows = _seen(spans, n)
+        for m, x in enumerate((q, k, v, dout)):
+            x.copy_(_rand(x.shape, BF16, 10 * i + m))
+            x[:, ~(keys if m in (1, 2) else rows)[0]] = math.nan
+        want = step()
+        if i % 2:
+            torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) and x.isnan().sum() == 0 for x, y in zip(got, want)), kind
