@@ -202,7 +202,9 @@ class Adam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work, entries = [], {}                                  # entries: of each parameter, so far
+        work, entries = [], {}                                  # entries: of each parameter, so far, where some are listed twice
+        listed = [id(p) for group in self.param_groups for p in group["params"]]
+        repeated = len(set(listed)) < len(listed)
         for group in self.param_groups:
             by_step = {}
             for p in group["params"]:
@@ -223,8 +225,11 @@ class Adam(torch.optim.Optimizer):
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 # a parameter that a group lists twice takes two steps, one launch behind the other: in one they would race
-                entries[p] = entries.get(p, 0) + 1
-                by_step.setdefault(int(st["step"].item()) + entries[p], []).append((p, g, st["exp_avg"], st["exp_avg_sq"]))
+                step = int(st["step"].item()) + 1
+                if repeated:
+                    step += entries.get(p, 0)
+                    entries[p] = entries.get(p, 0) + 1
+                by_step.setdefault(step, []).append((p, g, st["exp_avg"], st["exp_avg_sq"]))
             work += [(group, step, items) for step, items in sorted(by_step.items())]
         norm = None
         if self.max_grad_norm is not None and work:
