@@ -2,9 +2,9 @@
 //   D_i = sum_c dout_ic out_ic,  p_ij = exp(w_ij - lse_i),  dp_ij = dout_i . v_j,  ds_ij = scale (du/dt)_ij p_ij (dp_ij - D_i)
 //   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
 // in two kernels, each of which recomputes the scores: dq walks over keys with rows in registers, dk and dv over rows with keys in
-// registers. That is 7 products (for 16-bit types 8, as score gradients enter dq in two parts) for the 5 of a single kernel, whose dq would be added up with atomics in an order that changes
-// from call to call, and in fp32 memory that must be cleared before and converted behind. The gradient of a key/value head is
-// summed over the query heads that share it inside its workgroup.
+// registers. That is 7 products (for 16-bit types 8, as score gradients enter dq in two parts) for the 5 of a single kernel, whose dq
+// would be added up with atomics in an order that changes from call to call, and in fp32 memory that must be cleared before and
+// converted behind. The gradient of a key/value head is summed over the query heads that share it inside its workgroup.
 #include <algorithm>
 
 #include "span_attention.h"

@@ -236,7 +236,8 @@ int ddpm_sinusoidal_embedding(const void* t, int t_is_float, int batch, int emb_
 /* Rotary positions with several axes (time, height, width; one for a plain sequence): pair i of the axis_dim[a] channels
  * of axis a is turned by positions[token][a] * base^(-2 i / axis_dim[a]); the axes own consecutive channels from 0 on, and
  * channels behind the last axis pass unchanged. A pair is (i, axis_dim/2 + i) within its axis, or (2 i, 2 i + 1) with
- * interleaved != 0. inverse != 0 turns back: the gradient of the forward call. Angles are formed and reduced in float64 (off by 2^-51 of the position).
+ * interleaved != 0. inverse != 0 turns back: the gradient of the forward call. Angles are formed and reduced in float64, off by
+ * 2^-51 of the position.
  * One or two tensors (queries and keys of one sequence, own head counts) with the same positions; element (b, n, h, c) of
  * tensor i lies at x[i] + b*x_stride[i][0] + n*x_stride[i][1] + h*x_stride[i][2] + c, so that a channel slice of a fused
  * projection serves; out must not overlap x. positions: [batch or 1][tokens][axes], DDPM_I32, I64 or F32;
@@ -450,8 +451,8 @@ typedef struct ddpm_span_attention_args {
     void *dq, *dk, *dv;
     int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
     float* lse_near;                 /* like lse, of w with distances counted from the nearest key that the row sees: written by the
-                                        forward call and read by the backward one; NULL: the gradients' weights come from lse, and are off
-                                        by 2^-24 |lse| of themselves where a bias makes that large */
+                                        forward call and read by the backward one; NULL: the gradients' weights come from lse, which a
+                                        large bias leaves few digits for them */
 } ddpm_span_attention_args;
 
 /* Bytes of workspace (16-byte aligned, contents unspecified afterwards) of the two calls; negative for bad arguments.
